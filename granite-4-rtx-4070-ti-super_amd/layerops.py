@@ -141,6 +141,13 @@ _SIG = {
     "granite4_prefill_gemm_workspace_bytes": [I, I],
     "granite4_gemm_fp8_swiglu": [P, I, P, P, I, I, I, F, F, P, P, P, P],
     "granite4_gemm_fp8_residual_rmsnorm_fp8": [P, I, P, P, I, I, I, F, P, F, P, F, P, P, P],
+    "granite4_kv_ranges": [P, P, I, I, I, I, I, I, I, I, P, P, P, P, P, P],
+    "granite4_block_select_work_bytes": [I, I, I, I],
+    "granite4_block_select": [P, I, I, I, I, P, P, I, I, I, P, P, P, P, I, I, I, I, P, P],
+    "granite4_attn_blocks_scratch_bytes": [I, I, I, I],
+    "granite4_attn_blocks": [P, I, I, I, I, F, P, P, P, P, I, I, I, I, P, P, P, P, P, I, I, P, P],
+    "granite4_lora_work_bytes": [I, I, I, I, I, I],
+    "granite4_lora_add": [I, P, I, I, P, P, P, P, I, I, P, I, I, I, I, I, P, I, F, P, I, P],
     "granite4_kv_layout_offset": [Z, Z, Z, Z, Z, Z, I, Z, Z],
     "granite4_kv_pool_create": [Z, Z, Z, Z, Z],
     "granite4_kv_pool_destroy": [P],
@@ -203,7 +210,9 @@ _SIG = {
 }
 _RESTYPE = {"granite4_get_stream": P, "granite4_fp8_work_bytes": Z,
             "granite4_prefill_gemm_workspace_bytes": Z,
-            "granite4_attn_split_scratch_bytes": Z, "granite4_kv_pool_create": P,
+            "granite4_attn_split_scratch_bytes": Z, "granite4_block_select_work_bytes": Z,
+            "granite4_attn_blocks_scratch_bytes": Z, "granite4_lora_work_bytes": Z,
+            "granite4_kv_pool_create": P,
             "granite4_kv_ctrl_create": P}
 for _name, _args in _SIG.items():
     if os.environ.get("G4_LAYEROPS_LIB") and not hasattr(_lib, _name):
@@ -594,6 +603,81 @@ def rope_append(arena, q, k, v, cos, sin, base_pos=0, pos_rows=None, d_pt=None,
          0 if q_rot is None else q_rot.stride(0), arena.k, arena.v, arena.k_scale,
          arena.v_scale, arena.stride)
     return q_rot
+
+
+class KvRanges:
+    """The key ranges of one layer's arena (granite4_kv_ranges): codes int8
+    [Hk][stride / block][2][128] (lowest, highest) and their scales."""
+
+    def __init__(self, Hk, stride, block, device="cuda"):
+        self.Hk, self.stride, self.block = Hk, stride, block
+        self.codes = torch.zeros((Hk, stride // block, 2, 128), dtype=torch.int8, device=device)
+        self.scale = torch.zeros((Hk, stride // block), dtype=torch.float32, device=device)
+
+
+def kv_ranges(arena, ranges, rows, base_pos=0, d_pos=None, d_pt=None, row_pos=None, row_pt=None):
+    """The ranges of the blocks that end among the call's positions: `rows` of
+    one sequence from base_pos (or *d_pos) on, or row_pos[r] of each row."""
+    call("granite4_kv_ranges", arena.k, arena.k_scale, arena.bits, arena.group, arena.Hk, arena.d,
+         arena.stride, ranges.block, base_pos, rows, d_pos, d_pt, row_pos, row_pt, ranges.codes,
+         ranges.scale)
+    return ranges
+
+
+def block_select(q, ranges, top_k, sink=1, recent=2, base_pos=0, d_pos=None, d_pt=None,
+                 row_pos=None, row_pt=None, max_len=0, work=None, sel=None):
+    """granite4_block_select for q [rows][Hq * 128] bf16: the listed blocks
+    int32 [rows][Hk][top_k]."""
+    rows = q.shape[0]
+    if work is None:
+        work = torch.empty(call_size("granite4_block_select_work_bytes", rows, ranges.Hk,
+                                     max_len or ranges.stride, ranges.block), dtype=torch.uint8,
+                           device=q.device)
+    if sel is None:
+        sel = torch.empty((rows, ranges.Hk, top_k), dtype=torch.int32, device=q.device)
+    call("granite4_block_select", q, rows, q.shape[1] // 128, ranges.Hk, 128, ranges.codes,
+         ranges.scale, ranges.stride, ranges.block, base_pos, d_pos, d_pt, row_pos, row_pt,
+         max_len, top_k, sink, recent, work, sel)
+    return sel
+
+
+def attn_blocks(q, arena, sel, block, scale, base_pos=0, d_pos=None, d_pt=None, row_pos=None,
+                row_pt=None, scratch=None, out=None):
+    """granite4_attn_blocks for q [rows][Hq * 128] bf16 over the blocks listed
+    in sel [rows][Hk][top_k]."""
+    rows, top_k = q.shape[0], sel.shape[-1]
+    hq = q.shape[1] // arena.d
+    if scratch is None:
+        scratch = torch.empty(call_size("granite4_attn_blocks_scratch_bytes", hq, rows, top_k,
+                                        block), dtype=torch.uint8, device=q.device)
+    out = torch.empty_like(q) if out is None else out
+    call("granite4_attn_blocks", q, rows, hq, arena.Hk, arena.d, scale, arena.k, arena.v,
+         arena.k_scale, arena.v_scale, arena.bits, arena.group, arena.stride, base_pos, d_pos,
+         d_pt, row_pos, row_pt, sel, top_k, block, scratch, out)
+    return out
+
+
+def lora_add(x, A, B, alpha, row_adapter, base=None, segs=None, mult=1.0, x_scale=None, out=None,
+             work=None):
+    """granite4_lora_add: x [M][K] bf16 (or e4m3 codes, uint8, with a device
+    x_scale), A [adapters][parts][rank][K] and B [adapters][N][rank] bf16, alpha
+    f32 [adapters], row_adapter int32 [M]. base and the result are [M][N], bf16
+    or f32 (base None: bf16 unless out says otherwise); out may be base."""
+    M, K = x.shape
+    count, _, rank, _ = A.shape
+    N = B.shape[1]
+    s1, s2 = segs if segs is not None else (N, N)
+    if out is None:
+        out = torch.empty((M, N), dtype=torch.bfloat16 if base is None else base.dtype,
+                          device=x.device)
+    if work is None:
+        work = torch.empty(call_size("granite4_lora_work_bytes", M, N, K, rank, s1, s2),
+                           dtype=torch.uint8, device=x.device)
+    call("granite4_lora_add", GEMM_F32 if out.dtype == torch.float32 else GEMM_BF16, x,
+         8 if x_scale is not None else 16, x.stride(0), x_scale, A, B, alpha, count, rank,
+         row_adapter, M, N, K, int(s1), int(s2), base, 0 if base is None else base.stride(0),
+         float(mult), out, out.stride(0), work)
+    return out
 
 
 def multi_rows_struct():

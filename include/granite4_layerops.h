@@ -560,6 +560,109 @@ int granite4_gemm_fp8_residual_rmsnorm_fp8(const uint8_t* A, int lda, const floa
                                            float* d_scale, void* d_work);
 
 /* ---------------------------------------------------------------------------
+ * Block-sparse attention over the pool (no reference counterpart): a long
+ * context is cut into blocks of `block` positions (16, 32, 64 or 128); each
+ * query row and KV head attends to the top_k blocks that a cheap score finds
+ * for it. Three calls: granite4_kv_ranges after the append, granite4_block_select,
+ * granite4_attn_blocks. All three take rows of one sequence (row r at position
+ * kv_base + r, or *d_pos + r when d_pos is given; page table d_pt, NULL: row =
+ * position) or rows of sequences with their own positions and tables (row_pos
+ * and row_pt, both or neither; row_pt[r] may be NULL), are asynchronous on the
+ * calling thread's stream, allocate nothing and can be captured. d = 128,
+ * Hq = 4 Hk; bits, group, caches and scales as granite4_attn_paged; stride is
+ * a multiple of block; pointers to bf16 data, caches, ranges and workspaces
+ * are 16-byte aligned. A position read from device memory is clamped to the
+ * arena, table entries outside [0, stride) are passed over.
+ * ------------------------------------------------------------------------- */
+
+/* The ranges of every block whose last position is among the call's positions
+ * (the `rows` of one sequence, or each row_pos[r]): for block b in KV head h,
+ * lo and hi = the smallest and largest of each channel over the block's cached
+ * keys (code * scale in f32 for the quantised formats), as codes =
+ * clamp(round half away(x / s), +-127) under s = max(|lo|, |hi|) / 127 over the
+ * channels (s = 0: codes 0). ranges is [Hk][stride / block][2][128] int8 (lo,
+ * then hi), range_scale f32 [Hk][stride / block], indexed by the arena block
+ * that the block's first position begins, d_pt[b * block] / block: pages hold
+ * whole blocks (tokens_per_page a multiple of block), and sequences that share
+ * a page share its ranges. A block that begins elsewhere in the arena, or
+ * nowhere, gets none; blocks that the call does not complete keep theirs. A key
+ * without an arena row and a NaN element are passed over. */
+int granite4_kv_ranges(const void* cache_k, const float* k_scale, int bits, int group, int Hk,
+                       int d, int stride, int block, int base_pos, int rows, const int* d_pos,
+                       const int* d_pt, const int* row_pos, const int* const* row_pt,
+                       int8_t* ranges, float* range_scale);
+
+/* The blocks of each (row, KV head): sel [rows][Hk][top_k], ascending block
+ * numbers of the row's own sequence, -1 behind the last. A row at position p
+ * chooses among blocks 0 .. p / block. The first `sink` and the last `recent`
+ * (>= 1, so the row's own, perhaps unfinished, block) are listed always, the
+ * others by score, equal scores by the lower number:
+ *   score = max over the KV head's 4 query heads of (dot * s_b) * s_q,
+ *   dot = sum_d (qc_d < 0 ? qc_d lo_d : qc_d hi_d)   (the larger of the two, as lo <= hi)
+ * with the query head's codes qc = clamp(round half away(q / s_q), +-127),
+ * s_q = max|q| / 127, and the block's ranges and scale s_b. dot is a whole
+ * number, exact in f32, and the score has two f32 roundings: lists do not
+ * depend on how many rows a call has. A NaN score ranks lowest. Blocks without
+ * ranges (granite4_kv_ranges: off the arena, or beginning inside an arena
+ * block) are never listed. sink + recent <= top_k. max_len (0: stride) bounds
+ * the positions and sizes the work; positions behind it are clamped to it.
+ * work: granite4_block_select_work_bytes(rows, Hk, max_len, block) bytes (at
+ * most 64 MB but for contexts whose 16 rows need more), one call at a time. */
+size_t granite4_block_select_work_bytes(int rows, int Hk, int max_len, int block);
+int granite4_block_select(const uint16_t* q, int rows, int Hq, int Hk, int d,
+                          const int8_t* ranges, const float* range_scale, int stride, int block,
+                          int kv_base, const int* d_pos, const int* d_pt, const int* row_pos,
+                          const int* const* row_pt, int max_len, int top_k, int sink, int recent,
+                          void* work, int32_t* sel);
+
+/* Attention of each row over the blocks listed for it: out [rows][Hq * d] =
+ * softmax(scale * q . k) v over the positions <= the row's own of the listed
+ * blocks. sel [rows][Hk][top_k] as granite4_block_select writes it, or any list:
+ * entries in any order, below 0 or behind the row's position ignored, one that
+ * is listed twice counts twice. A row with no key gets zeros. Logits, running
+ * maximum and sum are f32; probabilities are rounded to bf16 for the value
+ * product (times the row's V scale where there is one scale per row; groups of
+ * 32 / 64 read each element as bf16(code * scale)). scratch:
+ * granite4_attn_blocks_scratch_bytes(Hq, rows, top_k, block) bytes (0 where the
+ * rows alone fill the chip: scratch may then be NULL), one call at a time. */
+size_t granite4_attn_blocks_scratch_bytes(int Hq, int rows, int top_k, int block);
+int granite4_attn_blocks(const uint16_t* q, int rows, int Hq, int Hk, int d, float scale,
+                         const void* cache_k, const void* cache_v, const float* k_scale,
+                         const float* v_scale, int bits, int group, int stride, int kv_base,
+                         const int* d_pos, const int* d_pt, const int* row_pos,
+                         const int* const* row_pt, const int32_t* sel, int top_k, int block,
+                         void* scratch, uint16_t* out);
+
+/* Low-rank adapters of many requests beside a shared projection (no reference
+ * counterpart): to the output of granite4_prefill_gemm or granite4_gemm_fp8
+ * (`base`), each row's own adapter is added,
+ *   y[m][n] = base[m][n] + mult * alpha[a] * sum_r t[r] B[a][n][r],
+ *   t[r] = sum_k x[m][k] A[a][part(n)][r][k],   a = d_row_adapter[m].
+ * Rows whose adapter is outside [0, adapters) get y = base. Rows may name
+ * adapters in any order (a tile of rows of one adapter is fastest).
+ *   out      GRANITE4_GEMM_BF16 or GRANITE4_GEMM_F32: the type of base and y.
+ *   X        the projection's input: bf16 (x_bits 16), or e4m3 codes under
+ *            *d_x_scale (x_bits 8); row pitch ldx elements.
+ *   A, B     bf16 [adapters][parts][rank][K] and [adapters][N][rank]; rank a
+ *            multiple of 8 up to 128 (pad smaller ranks with zeros); alpha f32
+ *            [adapters] in device memory.
+ *   seg1/2   columns where the second and third weight block begin, as in
+ *            Granite4GemmEpilogue: >= N (INT32_MAX) for none, else a multiple of
+ *            64. parts = 1, 2 or 3 blocks of A, one per weight block.
+ *   base     NULL: 0. May be y (ldb == ldy), and must not overlap it otherwise.
+ *            mult: the residual multiplier of an O / down projection, or 1.
+ * K % 64 == 0, N, ldy and ldb % 8 == 0, ldx % 8 == 0 (fp8: 16), 16-byte aligned
+ * pointers, M <= 1048560. The sum is f32, rounded once to y; t is kept to 2^-17
+ * (two bf16 terms) between the two launches, in work:
+ * granite4_lora_work_bytes(M, N, K, rank, seg1, seg2) bytes, one call at a
+ * time. Capturable. */
+size_t granite4_lora_work_bytes(int M, int N, int K, int rank, int seg1, int seg2);
+int granite4_lora_add(int out, const void* X, int x_bits, int ldx, const float* d_x_scale,
+                      const uint16_t* A, const uint16_t* B, const float* d_alpha, int adapters,
+                      int rank, const int* d_row_adapter, int M, int N, int K, int seg1, int seg2,
+                      const void* base, int ldb, float mult, void* y, int ldy, void* work);
+
+/* ---------------------------------------------------------------------------
  * Batch-1 decode GEMVs (bf16 activation x fp8 e4m3 weight rows [N][K]) with
  * the decode step's non-GEMM ops fused in. y[n] = scale * sum_k fp8(W[n][k])
  * * a[k] in f32, as the reference's gemv_row_dequant (forward_gpu.cu:
