@@ -212,6 +212,7 @@ _RESTYPE = {"granite4_get_stream": P, "granite4_fp8_work_bytes": Z,
             "granite4_prefill_gemm_workspace_bytes": Z,
             "granite4_attn_split_scratch_bytes": Z, "granite4_block_select_work_bytes": Z,
             "granite4_attn_blocks_scratch_bytes": Z, "granite4_lora_work_bytes": Z,
+            "granite4_kv_ranges": I,
             "granite4_kv_pool_create": P,
             "granite4_kv_ctrl_create": P}
 for _name, _args in _SIG.items():
