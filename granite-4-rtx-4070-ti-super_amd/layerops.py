@@ -233,6 +233,7 @@ for _name, _args in _SIG.items():
         _fn.restype = I
 
 lib = _lib
+_Tensor = torch.Tensor
 
 
 def _ptr(t):
@@ -250,8 +251,9 @@ def _check(rc, name):
 
 def call(name, *args):
     """Calls a C entry point by name; tensors are passed as device pointers."""
-    conv = [(_ptr(a) if (a is None or isinstance(a, torch.Tensor)) else a) for a in args]
-    _check(getattr(_lib, name)(*conv), name)
+    rc = getattr(_lib, name)(*[a.data_ptr() if isinstance(a, _Tensor) else a for a in args])
+    if rc != 0:
+        raise Granite4Error(f"{name} returned {rc}")
 
 
 def call_size(name, *args):
@@ -259,11 +261,19 @@ def call_size(name, *args):
     return getattr(_lib, name)(*args)
 
 
+_STREAM_LEGACY = 1  # hipStreamLegacy: the null stream by a handle of its own
+
+
 def use_stream(stream=None):
-    """Launch on `stream` (a torch.cuda.Stream) or torch's current stream."""
+    """Launch on `stream` (a torch.cuda.Stream) or torch's current stream. Torch's
+    default stream is the null stream, whose handle 0 granite4_set_stream takes
+    for the library's own default (the per-thread stream): named by its other
+    handle, the library's launches and torch's follow one another on it, where
+    every change between the two streams costs a wait for the device (a norm and
+    a torch operation in turn 43 us, on one stream 9)."""
     if stream is None:
         stream = torch.cuda.current_stream()
-    _lib.granite4_set_stream(stream.cuda_stream)
+    _lib.granite4_set_stream(stream.cuda_stream or _STREAM_LEGACY)
 
 
 def set_fp8_launch_mode(mode):
