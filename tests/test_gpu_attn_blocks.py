@@ -192,6 +192,21 @@ def test_select_chunk(rows, block, top_k, sink, recent):
     np.testing.assert_array_equal(got, lists(P, q, np.arange(rows), [pt] * rows, top_k, sink, recent))
 
 
+@pytest.mark.parametrize("rows,stride", [(9, 1 << 15), (3, 1 << 17), (2, 20480)])
+def test_select_rows_of_a_long_sequence(rows, stride):
+    P = Pool(16, 128, 1, 16, 16, 8)
+    P.stride = stride
+    n = stride // 16
+    P.rc = P.rng.integers(-127, 128, (1, n, 2, D)).astype(np.int8)
+    P.rs = (P.rng.random((1, n)) + 0.5).astype(np.float32)
+    P.drc, P.drs = dev(P.rc), dev(P.rs)
+    pt = ref.table(P.rng, n, 16)
+    q = queries(P.rng, rows, 1)
+    for start in (stride - rows, stride // 2 - 3):
+        got = P.select(q, start, dev(pt), top_k=70, sink=1, recent=2)
+        np.testing.assert_array_equal(got, lists(P, q, start + np.arange(rows), [pt] * rows, 70, 1, 2))
+
+
 def test_select_sessions_and_edges():
     P = Pool(16, 128, 3, 2048, 32, 11)
     a, b = ref.table(P.rng, 64, 32), ref.table(P.rng, 64, 32)
@@ -235,19 +250,20 @@ def test_select_ties_zero_and_not_finite():
     np.testing.assert_array_equal(got[1:], want[1:])
 
 
-def test_select_many_rows_share_a_bounded_workspace():
-    """16384 keys a row: the rows' scores are made some at a time."""
+@pytest.mark.parametrize("stride,rows", [(1 << 18, 1100), (1 << 20, 300)])
+def test_select_long_arena(stride, rows):
+    """16384 keys a row, which one workgroup holds, and 65536: scores in memory,
+    those of some of the rows at a time."""
     P = Pool(16, 128, 1, 16, 16, 6)
-    P.stride = 1 << 18
+    P.stride = stride
     n = P.stride // 16
     P.rc = P.rng.integers(-127, 128, (1, n, 2, D)).astype(np.int8)
     P.rs = (P.rng.random((1, n)) + 0.5).astype(np.float32)
     P.drc, P.drs = dev(P.rc), dev(P.rs)
-    rows = 1100
     assert L.call_size("granite4_block_select_work_bytes", rows, 1, P.stride, 16) < rows * n * 4
     q = queries(P.rng, rows, 1)
     got = P.select(q, 700, top_k=12, sink=1, recent=2)
-    at = [0, 511, 1023, 1024, 1027, 1099]
+    at = [0, 127, 255, 256, 259, rows - 1]
     want = lists(P, q[at], 700 + np.array(at), [np.arange(P.stride)] * len(at), 12, 1, 2)
     np.testing.assert_array_equal(got[at], want)
     # the longest context: every key of the arena
