@@ -16,8 +16,11 @@
 // as the dense decode attention (attn.hip) does. The running maximum and sum
 // and the logits stay in f32 (base 2, scale log2(e) folded into one factor); p
 // is rounded to bf16 for the value product, after its row's V scale.
+// Codes go into the products as they are: a scale group of K is one to four of
+// the 32-channel products, whose sum it scales, and p takes the V scale of each
+// group before its rounding, so no element of the cache is rounded again.
 // The four waves of a workgroup join in LDS, the workgroups of a row (splits,
-// where rows alone do not fill the chip) by a second launch.
+// where rows alone do not fill the chip) through memory, in the last of them.
 #include "attn_kv.h"
 #include "attn_rows.h"
 #include "g4_common.h"
@@ -46,6 +49,7 @@ struct BlocksArgs {
   RowSet at;
   const int32_t* sel;  // [rows][Hk][top_k]
   int top_k, log_block, splits;
+  unsigned* arrived;   // [rows][Hk] workgroups of the row that are done; 0 between calls
   float2* part_ml;     // [rows][Hq][splits]
   float* part_o;       // [rows][Hq][splits][128]
   uint16_t* out;       // [rows][Hq][128]
@@ -58,8 +62,7 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2))
 void attn_blocks_kernel(BlocksArgs a) {
   constexpr bool kQuant = BITS != 16;
   constexpr int kNgrp = kQuant ? kHd / GROUP : 1;
-  constexpr bool kDeq = kv_deq<BITS, GROUP>();
-  constexpr bool kQB = kQuant && !kDeq;  // the products see codes and row scales
+  constexpr int kSteps = 4 / kNgrp;  // 32-channel product steps per K scale
   constexpr int kKb = k_row_bytes(BITS), kVb = v_row_bytes(BITS);
   __shared__ __align__(16) uint16_t vl_all[kWaves][kTile * kVPitch];
   static_assert(2 * kNgrp * sizeof(float) <= (kVPitch - kHd) * sizeof(uint16_t), "scales in the pad");
@@ -150,10 +153,6 @@ void attn_blocks_kernel(BlocksArgs a) {
     if constexpr (kVDma) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       v_fix_bf16(vl, kvalid);
-    } else if constexpr (kDeq) {
-      store_scales();
-      wave_lds_sync();
-      v_store_deq<BITS, GROUP>(vraw, vl, kvalid, vsc_at);
     } else {
       v_store<BITS>(vraw, vl, kvalid);
       store_scales();
@@ -164,21 +163,27 @@ void attn_blocks_kernel(BlocksArgs a) {
 #pragma unroll
     for (int mb = 0; mb < 4; ++mb) {
       bf16x8_t ka[4];
-      if constexpr (kDeq) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s) ka[s] = k_raw_deq<BITS>(kraw[mb][s], ksc_at(16 * mb + n, (32 * s) / GROUP));
-      } else {
+      for (int s = 0; s < 4; ++s) ka[s] = k_raw_bf16<BITS>(kraw[mb][s]);
+      // q . codes of each scale group, then its scale
+      f32x4_t x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int s = 0; s < 4; ++s) ka[s] = k_raw_bf16<BITS>(kraw[mb][s]);
+      for (int gi = 0; gi < kNgrp; ++gi) {
+        f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka[kSteps * gi + s], qb[kSteps * gi + s], acc, 0, 0, 0);
+        if constexpr (!kQuant) {
+          x = acc;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = fmaf(acc[i], ksc_at(16 * mb + 4 * g + i, gi), x[i]);
+        }
       }
-      f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int s = 0; s < 4; ++s) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka[s], qb[s], acc, 0, 0, 0);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int key = 16 * mb + 4 * g + i;
-        const float x = kQB ? acc[i] * ksc_at(key, 0) : acc[i];
-        sv[mb][i] = live && ((kvalid >> key) & 1ull) ? a.scale2 * x : -INFINITY;
+        sv[mb][i] = live && ((kvalid >> key) & 1ull) ? a.scale2 * x[i] : -INFINITY;
       }
     }
     float mx = m;
@@ -203,14 +208,18 @@ void attn_blocks_kernel(BlocksArgs a) {
       }
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      float pv[8];
+      bf16x8_t pb[kNgrp];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int mb = 2 * s + (j >> 2), i = j & 3;
-        pv[j] = e[mb][i] * (kQB ? vsc_at(16 * mb + 4 * g + i, 0) : 1.0f);
+      for (int gi = 0; gi < kNgrp; ++gi) {
+        float pv[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int mb = 2 * s + (j >> 2), i = j & 3;
+          pv[j] = e[mb][i] * (kQuant ? vsc_at(16 * mb + 4 * g + i, gi) : 1.0f);
+        }
+        pb[gi] = as_bf16x8(pack_bf16_hw(pv[0], pv[1]), pack_bf16_hw(pv[2], pv[3]), pack_bf16_hw(pv[4], pv[5]),
+                           pack_bf16_hw(pv[6], pv[7]));
       }
-      const bf16x8_t pb = as_bf16x8(pack_bf16_hw(pv[0], pv[1]), pack_bf16_hw(pv[2], pv[3]),
-                                    pack_bf16_hw(pv[4], pv[5]), pack_bf16_hw(pv[6], pv[7]));
       const int kk = n >> 2, dd = 4 * (n & 3);
       const int vrow = 32 * s + 4 * g + kk;
       const uint16_t* r1 = vl + vrow * (kVDma ? kHd : kVPitch) + dd;
@@ -221,7 +230,8 @@ void attn_blocks_kernel(BlocksArgs a) {
         const int co = kVDma ? 16 * (nb ^ vt) : 16 * nb;
         const u32x2_t lo = lds_read_tr(r1 + co);
         const u32x2_t hi = lds_read_tr(r2 + co);
-        o[nb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(lo.x, lo.y, hi.x, hi.y), pb, o[nb], 0, 0, 0);
+        o[nb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(lo.x, lo.y, hi.x, hi.y), pb[kQuant ? (16 * nb) / GROUP : 0],
+                                                        o[nb], 0, 0, 0);
       }
     }
     wave_lds_sync();  // this tile's LDS reads are done before the next tile's writes
@@ -263,27 +273,43 @@ void attn_blocks_kernel(BlocksArgs a) {
     return;
   }
   const size_t at = rh * a.splits + split;
-  if (lane == 0) a.part_ml[at] = make_float2(M, L);
-  *reinterpret_cast<float2*>(a.part_o + at * kHd + 2 * lane) = make_float2(a0, a1);
-}
-
-// One wave per (row, head): its splits joined, in order.
-__global__ __launch_bounds__(256) void attn_blocks_join_kernel(BlocksArgs a) {
-  const int lane = threadIdx.x & 63;
-  const size_t rh = static_cast<size_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (rh >= static_cast<size_t>(a.rows) * kGq * a.Hk) return;
-  float M = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.part_ml[rh * a.splits + s].x);
-  float L = 0.0f, a0 = 0.0f, a1 = 0.0f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float2 ml = a.part_ml[rh * a.splits + s];
-    const float wt = ml.x == -INFINITY ? 0.0f : exp2_hw(ml.x - M);
-    const float2 ow = *reinterpret_cast<const float2*>(a.part_o + (rh * a.splits + s) * kHd + 2 * lane);
-    L += ml.y * wt;
-    a0 += ow.x * wt;
-    a1 += ow.y * wt;
+  if (lane == 0) st_dev_u64(a.part_ml + at, f2_bits(M, L));
+  st_dev_u64(a.part_o + at * kHd + 2 * lane, f2_bits(a0, a1));
+  // The last of the row's workgroups to arrive joins them all: none waits. The
+  // join runs over the splits in order, whichever workgroup does it.
+  __shared__ unsigned s_arrived;
+  wait_stores();
+  __syncthreads();
+  unsigned* count = a.arrived + static_cast<size_t>(row) * a.Hk + h;
+  if (threadIdx.x == 0) s_arrived = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (s_arrived != static_cast<unsigned>(a.splits) - 1u) return;
+  if (threadIdx.x == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  const float2* pml = a.part_ml + rh * a.splits;
+  const float* po = a.part_o + rh * a.splits * kHd + 2 * lane;
+  // Lane s (mod 32) has split s's maximum and sum; eight splits' sums load at once.
+  static_assert(kMaxSplits <= 32, "a lane per split");
+  const unsigned long long mlb = ld_dev_u64(pml + min(lane & 31, a.splits - 1));
+  const float ms = __uint_as_float(static_cast<unsigned>(mlb)), ls = __uint_as_float(static_cast<unsigned>(mlb >> 32));
+  const float Mall = wave_max(ms);  // repeated lanes change no maximum
+  const float ws = ms == -INFINITY ? 0.0f : exp2_hw(ms - Mall);
+  L = a0 = a1 = 0.0f;
+#pragma unroll 1
+  for (int s0 = 0; s0 < a.splits; s0 += 8) {
+    unsigned long long ov[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ov[j] = ld_dev_u64(po + static_cast<size_t>(min(s0 + j, a.splits - 1)) * kHd);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (s0 + j < a.splits) {
+        const float wt = readlane_f32(ws, s0 + j);
+        L += readlane_f32(ls, s0 + j) * wt;
+        a0 += __uint_as_float(static_cast<unsigned>(ov[j])) * wt;
+        a1 += __uint_as_float(static_cast<unsigned>(ov[j] >> 32)) * wt;
+      }
+    }
   }
-  const float inv = M == -INFINITY ? 0.0f : 1.0f / L;
+  const float inv = Mall == -INFINITY ? 0.0f : 1.0f / L;
   *reinterpret_cast<uint32_t*>(a.out + rh * kHd + 2 * lane) = pack_bf16_hw(a0 * inv, a1 * inv);
 }
 
@@ -307,6 +333,8 @@ void launch_blocks(const BlocksArgs& a, int group, dim3 grid, hipStream_t st) {
   }
 }
 
+size_t arrived_bytes(int rows, int Hk) { return (static_cast<size_t>(rows) * Hk * sizeof(unsigned) + 255) / 256 * 256; }
+
 constexpr int kSlab = 65535;  // rows of one launch (grid.y)
 
 }  // namespace
@@ -319,7 +347,9 @@ extern "C" {
 size_t granite4_attn_blocks_scratch_bytes(int Hq, int rows, int top_k, int block) {
   if (Hq <= 0 || Hq % kGq != 0 || rows <= 0 || top_k <= 0 || block <= 0) return 0;
   const int splits = blocks_splits(rows, Hq / kGq, top_k, block);
-  return splits == 1 ? 0 : static_cast<size_t>(rows) * Hq * splits * (sizeof(float2) + kHd * sizeof(float));
+  return splits == 1 ? 0
+                     : arrived_bytes(rows, Hq / kGq) +
+                           static_cast<size_t>(rows) * Hq * splits * (sizeof(float2) + kHd * sizeof(float));
 }
 
 int granite4_attn_blocks(const uint16_t* q, int rows, int Hq, int Hk, int d, float scale,
@@ -357,18 +387,17 @@ int granite4_attn_blocks(const uint16_t* q, int rows, int Hq, int Hk, int d, flo
     a.q = q + static_cast<size_t>(r0) * Hq * kHd;
     a.sel = sel + static_cast<size_t>(r0) * Hk * top_k;
     a.out = out + static_cast<size_t>(r0) * Hq * kHd;
-    a.part_o = static_cast<float*>(scratch);
-    a.part_ml = reinterpret_cast<float2*>(a.part_o + static_cast<size_t>(a.rows) * Hq * a.splits * kHd);
+    if (a.splits > 1) {  // one slab
+      a.arrived = static_cast<unsigned*>(scratch);
+      a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(scratch) + arrived_bytes(a.rows, Hk));
+      a.part_o = reinterpret_cast<float*>(a.part_ml + static_cast<size_t>(a.rows) * Hq * a.splits);
+    }
     const dim3 grid(Hk, a.rows, a.splits);
     switch (bits) {
       case 16: launch_blocks<16>(a, group, grid, st); break;
       case 8: launch_blocks<8>(a, group, grid, st); break;
       case 4: launch_blocks<4>(a, group, grid, st); break;
       default: launch_blocks<5>(a, group, grid, st); break;
-    }
-    if (a.splits > 1) {
-      const unsigned waves = static_cast<unsigned>(a.rows) * Hq;
-      hipLaunchKernelGGL(attn_blocks_join_kernel, (waves + 3) / 4, 256, 0, st, a);
     }
   }
   return launch_status("granite4_attn_blocks");

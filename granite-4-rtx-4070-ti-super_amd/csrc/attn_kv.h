@@ -355,6 +355,24 @@ __device__ __forceinline__ void v_store(const u32x4_t (&raw)[VStage<BITS>::kStep
 // (each wave owns its LDS tile, so no workgroup barrier is needed).
 __device__ __forceinline__ void wave_lds_sync() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
+// Partials and arrival tags are written and read at device scope (sc1 on
+// gfx950): the workgroup that combines may run on another XCD, whose L2
+// holds none of the writer's lines, and a tag must not be seen before the
+// partial it announces.
+__device__ __forceinline__ void st_dev_u64(void* p, unsigned long long v) {
+  __hip_atomic_store(static_cast<unsigned long long*>(p), v, __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ unsigned long long ld_dev_u64(const void* p) {
+  return __hip_atomic_load(static_cast<unsigned long long*>(const_cast<void*>(p)), __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ unsigned long long f2_bits(float x, float y) {
+  return static_cast<unsigned long long>(__float_as_uint(x)) |
+         (static_cast<unsigned long long>(__float_as_uint(y)) << 32);
+}
+__device__ __forceinline__ void wait_stores() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 }  // namespace
 }  // namespace g4
 

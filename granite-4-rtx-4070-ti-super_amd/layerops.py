@@ -655,11 +655,11 @@ def block_select(q, ranges, top_k, sink=1, recent=2, base_pos=0, d_pos=None, d_p
 def attn_blocks(q, arena, sel, block, scale, base_pos=0, d_pos=None, d_pt=None, row_pos=None,
                 row_pt=None, scratch=None, out=None):
     """granite4_attn_blocks for q [rows][Hq * 128] bf16 over the blocks listed
-    in sel [rows][Hk][top_k]."""
+    in sel [rows][Hk][top_k]; scratch zero-filled once."""
     rows, top_k = q.shape[0], sel.shape[-1]
     hq = q.shape[1] // arena.d
     if scratch is None:
-        scratch = torch.empty(call_size("granite4_attn_blocks_scratch_bytes", hq, rows, top_k,
+        scratch = torch.zeros(call_size("granite4_attn_blocks_scratch_bytes", hq, rows, top_k,
                                         block), dtype=torch.uint8, device=q.device)
     out = torch.empty_like(q) if out is None else out
     call("granite4_attn_blocks", q, rows, hq, arena.Hk, arena.d, scale, arena.k, arena.v,

@@ -621,10 +621,10 @@ int granite4_block_select(const uint16_t* q, int rows, int Hq, int Hk, int d,
  * entries in any order, below 0 or behind the row's position ignored, one that
  * is listed twice counts twice. A row with no key gets zeros. Logits, running
  * maximum and sum are f32; probabilities are rounded to bf16 for the value
- * product (times the row's V scale where there is one scale per row; groups of
- * 32 / 64 read each element as bf16(code * scale)). scratch:
+ * product, times the V scale of the element's group. scratch:
  * granite4_attn_blocks_scratch_bytes(Hq, rows, top_k, block) bytes (0 where the
- * rows alone fill the chip: scratch may then be NULL), one call at a time. */
+ * rows alone fill the chip: scratch may then be NULL), zero-filled once after
+ * its allocation and left so by every call; one call at a time. */
 size_t granite4_attn_blocks_scratch_bytes(int Hq, int rows, int top_k, int block);
 int granite4_attn_blocks(const uint16_t* q, int rows, int Hq, int Hk, int d, float scale,
                          const void* cache_k, const void* cache_v, const float* k_scale,

@@ -111,10 +111,9 @@ def attend(q, kval, vval, block, pos, pt, stride, sel, scale):
 
     The kernel rounds p (times the V scale) to bf16: 2^-8 of sum p |v|; the result:
     2^-8 of it; and sums logits and values in f32 (128 products; at most a few
-    thousand keys): 2^-15 of the absolute sums. Groups of 32 / 64 add the bf16
-    rounding of each element, of K through the logits: the caller widens it."""
+    thousand keys): 2^-15 of the absolute sums."""
     Hk = kval.shape[0]
-    out, tol, lmax = np.zeros((4 * Hk, D)), np.zeros((4 * Hk, D)), np.zeros(4 * Hk)
+    out, tol = np.zeros((4 * Hk, D)), np.zeros((4 * Hk, D))
     for h in range(Hk):
         p = (sel[h].astype(np.int64)[:, None] * block + np.arange(block)).reshape(-1)
         p = p[(np.repeat(sel[h], block) >= 0) & (p <= pos)]
@@ -130,10 +129,10 @@ def attend(q, kval, vval, block, pos, pt, stride, sel, scale):
             w /= w.sum()
             out[4 * h + g] = w @ vval[h, r]
             mass = w @ np.abs(vval[h, r])
-            lmax[4 * h + g] = abs(scale) * (np.abs(kval[h, r]) @ np.abs(x)).max()
-            tol[4 * h + g] = 2.0 ** -8 * (mass + np.abs(out[4 * h + g])) + 2.0 ** -15 * (1 + lmax[4 * h + g]) * mass
+            lmax = abs(scale) * (np.abs(kval[h, r]) @ np.abs(x)).max()
+            tol[4 * h + g] = 2.0 ** -8 * (mass + np.abs(out[4 * h + g])) + 2.0 ** -15 * (1 + lmax) * mass
             tol[4 * h + g] += 1e-30
-    return out, tol, lmax
+    return out, tol
 
 
 def lora(x, A, B, alpha, adapter, base, segs, mult):
