@@ -333,7 +333,9 @@ void launch_blocks(const BlocksArgs& a, int group, dim3 grid, hipStream_t st) {
   }
 }
 
-size_t arrived_bytes(int rows, int Hk) { return (static_cast<size_t>(rows) * Hk * sizeof(unsigned) + 255) / 256 * 256; }
+// The counts' place at the start of every scratch, whatever the call: splits are
+// several only below 512 (row, KV head) pairs.
+constexpr size_t kArrivedBytes = 2 * kCUs * sizeof(unsigned);
 
 constexpr int kSlab = 65535;  // rows of one launch (grid.y)
 
@@ -348,7 +350,7 @@ size_t granite4_attn_blocks_scratch_bytes(int Hq, int rows, int top_k, int block
   if (Hq <= 0 || Hq % kGq != 0 || rows <= 0 || top_k <= 0 || block <= 0) return 0;
   const int splits = blocks_splits(rows, Hq / kGq, top_k, block);
   return splits == 1 ? 0
-                     : arrived_bytes(rows, Hq / kGq) +
+                     : kArrivedBytes +
                            static_cast<size_t>(rows) * Hq * splits * (sizeof(float2) + kHd * sizeof(float));
 }
 
@@ -389,7 +391,7 @@ int granite4_attn_blocks(const uint16_t* q, int rows, int Hq, int Hk, int d, flo
     a.out = out + static_cast<size_t>(r0) * Hq * kHd;
     if (a.splits > 1) {  // one slab
       a.arrived = static_cast<unsigned*>(scratch);
-      a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(scratch) + arrived_bytes(a.rows, Hk));
+      a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(scratch) + kArrivedBytes);
       a.part_o = reinterpret_cast<float*>(a.part_ml + static_cast<size_t>(a.rows) * Hq * a.splits);
     }
     const dim3 grid(Hk, a.rows, a.splits);

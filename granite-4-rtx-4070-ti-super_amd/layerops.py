@@ -673,7 +673,8 @@ def lora_add(x, A, B, alpha, row_adapter, base=None, segs=None, mult=1.0, x_scal
     """granite4_lora_add: x [M][K] bf16 (or e4m3 codes, uint8, with a device
     x_scale), A [adapters][parts][rank][K] and B [adapters][N][rank] bf16, alpha
     f32 [adapters], row_adapter int32 [M]. base and the result are [M][N], bf16
-    or f32 (base None: bf16 unless out says otherwise); out may be base."""
+    or f32 (base None: bf16 unless out says otherwise); out may be base. work:
+    zero-filled once."""
     M, K = x.shape
     count, _, rank, _ = A.shape
     N = B.shape[1]
@@ -682,7 +683,7 @@ def lora_add(x, A, B, alpha, row_adapter, base=None, segs=None, mult=1.0, x_scal
         out = torch.empty((M, N), dtype=torch.bfloat16 if base is None else base.dtype,
                           device=x.device)
     if work is None:
-        work = torch.empty(call_size("granite4_lora_work_bytes", M, N, K, rank, s1, s2),
+        work = torch.zeros(call_size("granite4_lora_work_bytes", M, N, K, rank, s1, s2),
                            dtype=torch.uint8, device=x.device)
     call("granite4_lora_add", GEMM_F32 if out.dtype == torch.float32 else GEMM_BF16, x,
          8 if x_scale is not None else 16, x.stride(0), x_scale, A, B, alpha, count, rank,

@@ -624,7 +624,8 @@ int granite4_block_select(const uint16_t* q, int rows, int Hq, int Hk, int d,
  * product, times the V scale of the element's group. scratch:
  * granite4_attn_blocks_scratch_bytes(Hq, rows, top_k, block) bytes (0 where the
  * rows alone fill the chip: scratch may then be NULL), zero-filled once after
- * its allocation and left so by every call; one call at a time. */
+ * its allocation (every call leaves its first 2048 bytes zero). Calls of any
+ * shape may share one that is large enough, one call at a time. */
 size_t granite4_attn_blocks_scratch_bytes(int Hq, int rows, int top_k, int block);
 int granite4_attn_blocks(const uint16_t* q, int rows, int Hq, int Hk, int d, float scale,
                          const void* cache_k, const void* cache_v, const float* k_scale,
@@ -652,10 +653,12 @@ int granite4_attn_blocks(const uint16_t* q, int rows, int Hq, int Hk, int d, flo
  *   base     NULL: 0. May be y (ldb == ldy), and must not overlap it otherwise.
  *            mult: the residual multiplier of an O / down projection, or 1.
  * K % 64 == 0, N, ldy and ldb % 8 == 0, ldx % 8 == 0 (fp8: 16), 16-byte aligned
- * pointers, M <= 1048560. The sum is f32, rounded once to y; t is kept to 2^-17
- * (two bf16 terms) between the two launches, in work:
- * granite4_lora_work_bytes(M, N, K, rank, seg1, seg2) bytes, one call at a
- * time. Capturable. */
+ * pointers, M <= 1048560. The sum is f32, rounded once to y; between the
+ * two launches t is kept as a sum of bf16 terms (two for a bf16 y, which lose
+ * 2^-17 of it, three for an f32 y), in work:
+ * granite4_lora_work_bytes(M, N, K, rank, seg1, seg2) bytes, zero-filled once
+ * after its allocation (every call leaves its first 2048 bytes zero). Calls of
+ * any shape may share one that is large enough, one call at a time. Capturable. */
 size_t granite4_lora_work_bytes(int M, int N, int K, int rank, int seg1, int seg2);
 int granite4_lora_add(int out, const void* X, int x_bits, int ldx, const float* d_x_scale,
                       const uint16_t* A, const uint16_t* B, const float* d_alpha, int adapters,

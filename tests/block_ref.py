@@ -148,7 +148,7 @@ def lora(x, A, B, alpha, adapter, base, segs, mult):
         f = np.float64(mult) * alpha[a]
         for i in range(len(cut) - 1):
             t = A[a, i] @ x[m]
-            # f32 sums of K products, t as two bf16 terms (2^-16 of it), f32 sums of 2 R
+            # f32 sums of K products, t as two or three bf16 terms (2^-16 of it), f32 sums of 2 R
             # products, and the three roundings of base + (mult alpha) (.)
             dt = K * 2.0 ** -24 * (np.abs(A[a, i]) @ np.abs(x[m])) + 2.0 ** -16 * np.abs(t)
             b = B[a, cut[i]:cut[i + 1]]

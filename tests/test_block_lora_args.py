@@ -82,12 +82,15 @@ def test_workspace_sizes():
         assert f(*bad) == 0
     f = L.lib.granite4_attn_blocks_scratch_bytes
     assert f(32, 4096, 32, 64) == 0
-    assert f(32, 1, 32, 64) > 256 and (f(32, 1, 32, 64) - 256) % (32 * 130 * 4) == 0
+    assert f(32, 1, 32, 64) > 2048 and (f(32, 1, 32, 64) - 2048) % (32 * 130 * 4) == 0
     for bad in ((0, 1, 1, 16), (30, 1, 1, 16), (32, 0, 1, 16), (32, 1, 0, 16), (32, 1, 1, 0)):
         assert f(*bad) == 0
     f = L.lib.granite4_lora_work_bytes
     big = 2**31 - 1
-    assert f(5, 6144, 4096, 16, 4096, 5120) == 5 * 3 * 16 * 4
-    assert f(5, 6144, 4096, 16, 4096, big) == 5 * 2 * 16 * 4
-    assert f(1 << 20, 6144, 4096, 128, big, big) == (1 << 29)
+    # counts, three bf16 terms of t (16-row tiles, 32 ranks), a sum of t for each share of K
+    for k, shares in ((64, 1), (1024, 1), (2048, 2), (4096, 4), (12800, 8)):
+        more = 4 * shares if shares > 1 else 0
+        assert f(5, 6144, k, 16, 4096, 5120) == 2048 + 3 * (16 * 32 * 6 + 5 * 16 * more)
+        assert f(5, 6144, k, 16, 4096, big) == 2048 + 2 * (16 * 32 * 6 + 5 * 16 * more)
+    assert f(1 << 20, 6144, 4096, 128, big, big) == 2048 + (6 << 27)
     assert f(0, 64, 64, 16, big, big) == 0

@@ -69,7 +69,7 @@ class Pool:
         rows, top_k = q.shape[0], sel.shape[-1]
         n = L.call_size("granite4_attn_blocks_scratch_bytes", 4 * self.Hk, rows, top_k, self.block)
         # zeros where calls count, NaN where they put their sums
-        head = -(-rows * self.Hk * 4 // 256) * 256
+        head = 2048
         scratch = torch.full((n + 16,), 255, dtype=torch.uint8, device="cuda")
         scratch[:head if n else 0] = 0
         out = torch.full((rows + 1, 4 * self.Hk * D), 0x7FC1, dtype=torch.int16, device="cuda")

@@ -62,14 +62,14 @@ class Case:
         y = d_base if in_place else torch.full((self.M + 1, self.ldy), 77, dtype=t, device="cuda")
         ldy = self.ldb if in_place else self.ldy
         n = L.call_size("granite4_lora_work_bytes", self.M, self.N, self.K, self.rank, *self.segs)
-        assert n == 4 * self.M * self.parts * self.rank
         work = torch.full((n + 16,), 255, dtype=torch.uint8, device="cuda")  # NaN, were it read first
+        work[:2048] = 0  # where calls count
         L.call("granite4_lora_add", int(self.f32), dev(self.x), 8 if self.fp8 else 16, self.ldx,
                dev(np.array([self.xs])) if self.fp8 else None, dev(self.A), dev(self.B),
                dev(self.alpha), self.count, self.rank, dev(self.adapter), self.M, self.N, self.K,
                *self.segs, d_base if base else None, self.ldb if base else 0, mult, y, ldy, work)
         got = host(y)
-        assert (host(work)[n:] == 255).all()
+        assert (host(work)[n:] == 255).all() and (host(work)[:2048] == 0).all()
         if in_place:
             keep = self.base if self.f32 else self.base.view(np.int16)
             np.testing.assert_array_equal(got[:, self.N:], keep[:, self.N:])
@@ -182,7 +182,7 @@ def test_lora_in_a_graph_with_changing_rows():
         L.use_stream(s)
         x, A, B, alpha, base = (dev(t) for t in (c.x, c.A, c.B, c.alpha, c.base))
         adapter = dev(c.adapter)
-        work = torch.empty(L.call_size("granite4_lora_work_bytes", 16, 256, 256, 16, 64, 128),
+        work = torch.zeros(L.call_size("granite4_lora_work_bytes", 16, 256, 256, 16, 64, 128),
                            dtype=torch.uint8, device="cuda")
         y = torch.empty((16, 256), dtype=torch.int16, device="cuda")
 
