@@ -127,7 +127,7 @@ __device__ __forceinline__ void store_t(const LoraArgs& a, int m, int r, f32x4_t
 // 128 bytes of different banks). DS operations of a wave execute in order, so
 // the tiles of the next 32 follow without a wait.
 template <int RT, int XT, bool FP8>
-__global__ __launch_bounds__(kShrinkWaves * 64) __attribute__((amdgpu_waves_per_eu(4)))
+__global__ __launch_bounds__(kShrinkWaves * 64) __attribute__((amdgpu_waves_per_eu(RT * XT > 8 ? 2 : 4)))
 void lora_shrink_kernel(LoraArgs a) {
   constexpr int kXRows = 16 * XT;
   constexpr int kDeep = RT + XT <= 2 ? 4 : 2;  // units in flight: 128 registers a lane
@@ -380,7 +380,7 @@ struct Shrink {
 };
 Shrink shrink_plan(int M, int K, int pr, int adapters) {
   Shrink p;
-  p.xt = M <= 64 ? 1 : 2;
+  p.xt = M <= 64 ? 1 : M >= 4096 && pr > 32 ? 4 : 2;
   p.rt = M <= 64 || pr <= 16 ? 1 : pr <= 32 ? 2 : 4;
   // One tile's distinct adapters over workgroups of their own where rows are few.
   p.slots = M <= 64 ? std::min({16, M, adapters}) : 1;
@@ -486,7 +486,8 @@ int granite4_lora_add(int out, const void* X, int x_bits, int ldx, const float* 
   if (plan.xt == 1) launch_shrink<1, 1>(a, fp8, slots, st);
   else if (plan.rt == 1) launch_shrink<1, 2>(a, fp8, 1, st);
   else if (plan.rt == 2) launch_shrink<2, 2>(a, fp8, 1, st);
-  else launch_shrink<4, 2>(a, fp8, 1, st);
+  else if (plan.xt == 2) launch_shrink<4, 2>(a, fp8, 1, st);
+  else launch_shrink<4, 4>(a, fp8, 1, st);
   const int per = M <= 256 ? 1 : 4;
   const bool f32 = out == GRANITE4_GEMM_F32;
   const int steps = rank_steps(rank);
