@@ -198,7 +198,7 @@ __device__ __forceinline__ int row_blocks(const SelectArgs& a, int r) {
 //
 // Query codes are made once per workgroup, 16 lanes to a column, into LDS; a
 // wave then takes 64 blocks at a time: their table entries, one per lane, their
-// 256-byte code rows straight from memory as B of v_mfma_i32_16x16x64_i8
+// 256-byte code rows, 16 lanes to a row, through LDS as B of v_mfma_i32_16x16x64_i8
 // (K = 256: the lowest, then the highest codes), and A = the queries' negative,
 // then their positive codes: a lane gets the four heads of one row at one
 // block, and takes their maximum without another. put(rr, b, key) receives a key.
@@ -206,7 +206,7 @@ template <int W, int ROWS>
 struct Scorer {
   static constexpr int kTiles = (ROWS * 4 + 15) / 16;  // 16-column tiles
   static constexpr int kCols = ROWS * 4;
-  static constexpr int kLoads = ROWS > 4 ? 2 : 4;  // registers for four waves per SIMD
+  static constexpr int kLoads = 2;  // 16-block tiles in flight (4: 0.5 us more for one row, spills)
   // One more 16-byte unit per column, so that 16 columns' reads spread over the banks.
   static constexpr int kPitch = 9;
   static constexpr int kHold = kTiles <= 2 ? kTiles : 1;  // tiles whose query codes stay in registers
@@ -265,17 +265,26 @@ struct Scorer {
   // 64 blocks from b0 on, kLoads 16-block tiles' rows in flight at a time.
   template <bool PLAIN, class Put>
   __device__ __forceinline__ static void unit(const Shared& sh, const SelectArgs& a, int nr, size_t hb, int ab, float sb,
-                                              int b0, int row0,
+                                              int b0, int row0, i32x4_t* turn,
                                               const QFrag (&held)[kHold], Put put) {
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
 #pragma unroll 1
     for (int t0 = 0; t0 < 4; t0 += kLoads) {
       i32x4_t ka[kLoads][4];
 #pragma unroll
-      for (int t = 0; t < kLoads; ++t) {
-        const int8_t* src = a.ranges + (hb + __shfl(ab, 16 * (t0 + t) + n)) * 256 + 16 * g;
+      for (int t = 0; t < kLoads; ++t)
 #pragma unroll
-        for (int s = 0; s < 4; ++s) ka[t][s] = *reinterpret_cast<const i32x4_t*>(src + 64 * s);
+        for (int j = 0; j < 4; ++j)
+          ka[t][j] = *reinterpret_cast<const i32x4_t*>(a.ranges + (hb + __shfl(ab, 16 * (t0 + t) + 4 * j + g)) * 256 + 16 * n);
+      // Each tile through LDS into fragments: row r's 16-byte chunk c in slot c ^ r.
+#pragma unroll
+      for (int t = 0; t < kLoads; ++t) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) turn[16 * (4 * j + g) + (n ^ (4 * j + g))] = ka[t][j];
+        asm volatile("" ::: "memory");  // a wave's DS operations execute in order
+#pragma unroll
+        for (int s = 0; s < 4; ++s) ka[t][s] = turn[16 * n + ((4 * s + g) ^ n)];
+        asm volatile("" ::: "memory");
       }
       float sbt[kLoads];
 #pragma unroll
@@ -310,7 +319,7 @@ struct Scorer {
 
   template <class Put>
   __device__ __forceinline__ static void score(const Shared& sh, const SelectArgs& a, int h, int row0, int nr, int most,
-                               const int* pt, int first, int b0, int step, Put put) {
+                               const int* pt, int first, int b0, int step, i32x4_t* turn, Put put) {
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const size_t hb = static_cast<size_t>(h) * (a.stride >> a.log_block);
     const int have_least = row_blocks(a, row0);
@@ -329,8 +338,8 @@ struct Scorer {
       const float sb = there ? sb_mem : -1.0f;
       // Where every block of the unit is scored for every row, no key looks at more.
       const bool plain = nr == ROWS && b0 >= a.sink && b0 + 64 <= have_least - a.recent && __all(there);
-      if (plain) unit<true>(sh, a, nr, hb, ab, sb, b0, row0, held, put);
-      else unit<false>(sh, a, nr, hb, ab, sb, b0, row0, held, put);
+      if (plain) unit<true>(sh, a, nr, hb, ab, sb, b0, row0, turn, held, put);
+      else unit<false>(sh, a, nr, hb, ab, sb, b0, row0, turn, held, put);
       first = next;
     }
   }
@@ -605,6 +614,7 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(4))) voi
     __align__(16) WidePick<16, KEYS / 4096 + (KEYS < 4096)> wide;
   } u;
   __shared__ __align__(16) uint32_t keys[ROWS][KEYS];
+  __shared__ i32x4_t turn[W][256];
   const int wave = threadIdx.x >> 6;
   const int h = blockIdx.x, row0 = blockIdx.y * ROWS, nr = min(ROWS, a.rows - row0);
   const int most = most_blocks(a, row0, nr);
@@ -612,7 +622,7 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(4))) voi
   const int first = wave * 64 < most ? S::entry(a, pt, wave * 64, most) : -1;
   S::quantise(u.sh, a, h, row0, nr);
   __syncthreads();
-  S::score(u.sh, a, h, row0, nr, most, pt, first, wave * 64, W * 64,
+  S::score(u.sh, a, h, row0, nr, most, pt, first, wave * 64, W * 64, turn[wave],
            [&](int rr, int b, uint32_t k) { keys[rr][b] = k; });
   __syncthreads();
   if constexpr (ROWS == 1) {
@@ -637,6 +647,7 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(4))) voi
 __global__ __launch_bounds__(256) void block_score_kernel(SelectArgs a) {
   using S = Scorer<4, 4>;
   __shared__ S::Shared sh;
+  __shared__ i32x4_t turn[4][256];
   const int per = a.at.row_pos != nullptr ? 1 : 4;
   const int lr0 = blockIdx.x * per, nr = min(per, a.nrows - lr0), row0 = a.r0 + lr0;
   const int h = blockIdx.y, b0 = (blockIdx.z * 4 + (threadIdx.x >> 6)) * 64;
@@ -647,7 +658,7 @@ __global__ __launch_bounds__(256) void block_score_kernel(SelectArgs a) {
   S::quantise(sh, a, h, row0, nr);
   __syncthreads();
   uint32_t* dst = a.keys + (static_cast<size_t>(lr0) * a.Hk + h) * a.nbp;
-  S::score(sh, a, h, row0, nr, min(most, b0 + 1), pt, first, b0, 64, [&](int rr, int b, uint32_t k) {
+  S::score(sh, a, h, row0, nr, min(most, b0 + 1), pt, first, b0, 64, turn[threadIdx.x >> 6], [&](int rr, int b, uint32_t k) {
     dst[static_cast<size_t>(rr) * a.Hk * a.nbp + b] = k;
   });
 }
@@ -736,7 +747,7 @@ __global__ __launch_bounds__(256) void block_pick_kernel(SelectArgs a) {
 }
 
 // The most keys of a row that the one-launch form holds in LDS.
-constexpr int kLdsKeys = 32768;
+constexpr int kLdsKeys = 16384;
 
 template <int W, int ROWS, int KEYS>
 void launch_select(const SelectArgs& a, hipStream_t st) {
@@ -843,11 +854,10 @@ int granite4_block_select(const uint16_t* q, int rows, int Hq, int Hk, int d,
   a.sel = sel;
   const hipStream_t st = stream();
   const bool one_seq = row_pos == nullptr;
-  const long long groups = one_seq && rows > 1 ? (static_cast<long long>(rows) + 7) / 8 : rows;
+  const long long groups = one_seq && rows > 1 && a.nbp <= 4096 ? (static_cast<long long>(rows) + 3) / 4 : rows;
   if (a.nbp <= kLdsKeys && groups <= 65535) {
-    if (one_seq && a.nbp <= 1024 && (rows + 31) / 32 * Hk >= 192) launch_select<16, 32, 1024>(a, st);
-    else if (one_seq && rows > 1 && a.nbp <= 1024) launch_select<8, 8, 1024>(a, st);
-    else if (one_seq && rows > 1 && a.nbp <= 4096) launch_select<8, 8, 4096>(a, st);
+    if (one_seq && rows > 1 && a.nbp <= 1024) launch_select<8, 8, 1024>(a, st);
+    else if (one_seq && rows > 1 && a.nbp <= 4096) launch_select<16, 4, 4096>(a, st);
     else if (a.nbp <= 4096) launch_select<16, 1, 4096>(a, st);
     else launch_select<16, 1, kLdsKeys>(a, st);
     return launch_status("granite4_block_select");
