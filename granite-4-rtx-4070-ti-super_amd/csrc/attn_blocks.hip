@@ -11,9 +11,10 @@
 // page table puts them. One wave takes a tile with 16 MFMA columns, of which
 // the four heads fill 4: rows share no lists, so there is nothing to put into
 // the others, and a tile's bytes take longer than its products.
-//   S^T = K Q^T   v_mfma_f32_16x16x32_bf16, K rows straight from the pool
-//   O^T += V^T P^T  V through a row-major LDS tile, read transposed
-// as the dense decode attention (attn.hip) does. The running maximum and sum
+//   S^T = K Q^T   v_mfma_f32_16x16x32_bf16, K rows through a stage of LDS (KStage)
+//   O^T += V^T P^T  V through a row-major LDS tile, read transposed as the dense
+//                   decode attention (attn.hip) does.
+// The running maximum and sum
 // and the logits stay in f32 (base 2, scale log2(e) folded into one factor); p
 // is rounded to bf16 for the value product, after its row's V scale.
 // Codes go into the products as they are: a scale group of K is one to four of
@@ -57,6 +58,55 @@ struct BlocksArgs {
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// K rows of 16 keys on their way from memory (16-byte chunks, consecutive lanes
+// along a row) to fragments (lane n + 16 g: key n's channels 32 s + 8 g ..):
+// through a stage of LDS that a wave has to itself. Straight from memory a
+// quarter of a wave takes 16 bytes of each of 16 rows, 16 cache lines for 256
+// bytes, and the CU's cache gives a quarter of its rate. The chunks of row r are
+// exchanged (by r, r mod 8, r / 2 mod 4; K5 rows of 80 bytes need none), so that
+// reads meet different banks.
+template <int BITS>
+struct KStage {
+  static constexpr int kRow = k_row_bytes(BITS), kChunks = kRow / 16;  // per key: 16, 8, 4 or 5
+  static constexpr int kLoads = (16 * kChunks + 63) / 64;
+  static constexpr int kBytes = 16 * kRow;
+  static __device__ __forceinline__ int slot(int key, int c) {
+    if constexpr (BITS == 16) return c ^ key;
+    else if constexpr (BITS == 8) return c ^ (key & 7);
+    else if constexpr (BITS == 4) return c ^ ((key >> 1) & 3);
+    else return c;
+  }
+  // Load i of the 16 keys from `first` on; row_of(key): its arena row (any, where it has none).
+  template <class F>
+  static __device__ __forceinline__ u32x4_t load(const uint8_t* kbase, int first, int i, F row_of) {
+    const int id = i * 64 + (threadIdx.x & 63), key = min(id / kChunks, 15), c = id % kChunks;
+    return *reinterpret_cast<const u32x4_t*>(kbase + static_cast<size_t>(row_of(first + key)) * kRow + 16 * c);
+  }
+  static __device__ __forceinline__ void put(uint8_t* stage, int i, const u32x4_t& v) {
+    const int id = i * 64 + (threadIdx.x & 63), key = id / kChunks, c = id % kChunks;
+    if (16 * kChunks % 64 == 0 || key < 16) *reinterpret_cast<u32x4_t*>(stage + key * kRow + 16 * slot(key, c)) = v;
+  }
+  // load_k_raw's form of key n, channels 32 s + 8 g ..
+  static __device__ __forceinline__ u32x4_t get(const uint8_t* stage, int n, int s, int g) {
+    const uint8_t* row = stage + n * kRow;
+    u32x4_t r = {0u, 0u, 0u, 0u};
+    if constexpr (BITS == 16) {
+      r = *reinterpret_cast<const u32x4_t*>(row + 16 * slot(n, 4 * s + g));
+    } else if constexpr (BITS == 8) {
+      const u32x2_t v = *reinterpret_cast<const u32x2_t*>(row + 16 * slot(n, 2 * s + (g >> 1)) + 8 * (g & 1));
+      r.x = v.x;
+      r.y = v.y;
+    } else {
+      r.x = *reinterpret_cast<const uint32_t*>(row + 16 * slot(n, s) + 4 * g);
+      if constexpr (BITS == 5) r.y = row[kHd / 2 + 4 * s + g];
+    }
+    return r;
+  }
+};
+
+// Orders a wave's DS operations for the compiler; the hardware executes them in order.
+__device__ __forceinline__ void ds_in_order() { asm volatile("" ::: "memory"); }
+
 template <int BITS, int GROUP>
 __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2)))
 void attn_blocks_kernel(BlocksArgs a) {
@@ -64,10 +114,16 @@ void attn_blocks_kernel(BlocksArgs a) {
   constexpr int kNgrp = kQuant ? kHd / GROUP : 1;
   constexpr int kSteps = 4 / kNgrp;  // 32-channel product steps per K scale
   constexpr int kKb = k_row_bytes(BITS), kVb = v_row_bytes(BITS);
-  __shared__ __align__(16) uint16_t vl_all[kWaves][kTile * kVPitch];
+  using KS = KStage<BITS>;
+  constexpr bool kVDma = BITS == 16;  // V rows straight to LDS, without a pad
+  // Per wave the V tile and the K stage; two workgroups fill a CU's 160 KB.
+  constexpr int kVBytes = 2 * kTile * (kVDma ? kHd : kVPitch), kLdsWave = 20480;
+  static_assert(kVBytes + KS::kBytes <= kLdsWave, "a wave's LDS");
+  __shared__ __align__(16) uint8_t lds[kWaves][kLdsWave];
   static_assert(2 * kNgrp * sizeof(float) <= (kVPitch - kHd) * sizeof(uint16_t), "scales in the pad");
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint16_t* vl = vl_all[wave];
+  uint16_t* vl = reinterpret_cast<uint16_t*>(lds[wave]);
+  uint8_t* const stage = lds[wave] + kVBytes;
   float* const vlf = reinterpret_cast<float*>(vl);
   auto ksc_at = [&](int key, int gi) -> float& { return vlf[key * (kVPitch / 2) + kHd / 2 + gi]; };
   auto vsc_at = [&](int key, int gi) -> float& { return vlf[key * (kVPitch / 2) + kHd / 2 + 4 + gi]; };
@@ -120,18 +176,13 @@ void attn_blocks_kernel(BlocksArgs a) {
     const unsigned long long kvalid = __ballot(prow >= 0);
     if (t + step < tiles) prow_next = slot_row(t + step);
     if (kvalid == 0ull) continue;
-    constexpr bool kVDma = BITS == 16;
-    u32x4_t vraw[VStage<BITS>::kSteps];
-    if constexpr (kVDma) v_dma_bf16(vbase, prow, vl);
-    else v_load<BITS>(vbase, prow, vraw);
-    u32x4_t kraw[4][4];
+    // K and the scales first, then V, which lands while the logits are made.
+    u32x4_t kraw[4][KS::kLoads];
 #pragma unroll
-    for (int mb = 0; mb < 4; ++mb) {
-      const int kr = __shfl(prow, 16 * mb + n);
-      const uint8_t* krow = kbase + static_cast<size_t>(kr >= 0 ? kr : 0) * kKb;
+    for (int mb = 0; mb < 4; ++mb)
 #pragma unroll
-      for (int s = 0; s < 4; ++s) kraw[mb][s] = load_k_raw<BITS>(krow, 32 * s + 8 * g);
-    }
+      for (int i = 0; i < KS::kLoads; ++i)
+        kraw[mb][i] = KS::load(kbase, 16 * mb, i, [&](int key) { return max(__shfl(prow, key), 0); });
     float ksr[kNgrp], vsr[kNgrp];
     if constexpr (kQuant) {
 #pragma unroll
@@ -141,30 +192,27 @@ void attn_blocks_kernel(BlocksArgs a) {
         vsr[gi] = vscb[si];
       }
     }
-    const auto store_scales = [&] {
-      if constexpr (kQuant) {
+    u32x4_t vraw[VStage<BITS>::kSteps];
+    if constexpr (kVDma) v_dma_bf16(vbase, prow, vl);
+    else v_load<BITS>(vbase, prow, vraw);
+    if constexpr (kQuant) {
 #pragma unroll
-        for (int gi = 0; gi < kNgrp; ++gi) {
-          ksc_at(lane, gi) = prow >= 0 ? ksr[gi] : 0.0f;
-          vsc_at(lane, gi) = prow >= 0 ? vsr[gi] : 0.0f;
-        }
+      for (int gi = 0; gi < kNgrp; ++gi) {
+        ksc_at(lane, gi) = prow >= 0 ? ksr[gi] : 0.0f;
+        vsc_at(lane, gi) = prow >= 0 ? vsr[gi] : 0.0f;
       }
-    };
-    if constexpr (kVDma) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      v_fix_bf16(vl, kvalid);
-    } else {
-      v_store<BITS>(vraw, vl, kvalid);
-      store_scales();
     }
-    wave_lds_sync();
     // Keys 16 mb + 4 g + i of column n.
     float sv[4][4];
 #pragma unroll
     for (int mb = 0; mb < 4; ++mb) {
+#pragma unroll
+      for (int i = 0; i < KS::kLoads; ++i) KS::put(stage, i, kraw[mb][i]);
+      ds_in_order();
       bf16x8_t ka[4];
 #pragma unroll
-      for (int s = 0; s < 4; ++s) ka[s] = k_raw_bf16<BITS>(kraw[mb][s]);
+      for (int s = 0; s < 4; ++s) ka[s] = k_raw_bf16<BITS>(KS::get(stage, n, s, g));
+      ds_in_order();
       // q . codes of each scale group, then its scale
       f32x4_t x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -206,6 +254,13 @@ void attn_blocks_kernel(BlocksArgs a) {
         e[mb][i] = sv[mb][i] == -INFINITY ? 0.0f : exp2_hw(sv[mb][i] - m);
         l += e[mb][i];
       }
+    if constexpr (kVDma) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      v_fix_bf16(vl, kvalid);
+    } else {
+      v_store<BITS>(vraw, vl, kvalid);
+    }
+    ds_in_order();
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       bf16x8_t pb[kNgrp];
@@ -239,7 +294,7 @@ void attn_blocks_kernel(BlocksArgs a) {
   l = col_sum4(l);
   // The workgroup's waves joined: [wave][4 heads][128] and their (m, l).
   __syncthreads();
-  float* mo = reinterpret_cast<float*>(&vl_all[0][0]);
+  float* mo = reinterpret_cast<float*>(&lds[0][0]);
   float* mml = mo + kWaves * kGq * kHd;
   if (live) {
 #pragma unroll
@@ -277,7 +332,8 @@ void attn_blocks_kernel(BlocksArgs a) {
   st_dev_u64(a.part_o + at * kHd + 2 * lane, f2_bits(a0, a1));
   // The last of the row's workgroups to arrive joins them all: none waits. The
   // join runs over the splits in order, whichever workgroup does it.
-  __shared__ unsigned s_arrived;
+  unsigned& s_arrived = *reinterpret_cast<unsigned*>(&lds[kWaves - 1][0]);  // past the joined sums
+  static_assert(sizeof(float) * kWaves * kGq * (kHd + 2) <= (kWaves - 1) * kLdsWave, "room for the count");
   wait_stores();
   __syncthreads();
   unsigned* count = a.arrived + static_cast<size_t>(row) * a.Hk + h;
