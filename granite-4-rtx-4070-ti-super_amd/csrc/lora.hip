@@ -115,24 +115,24 @@ __device__ __forceinline__ void store_t(const LoraArgs& a, int m, int r, f32x4_t
 }
 
 // Workgroup: XT x 16 rows of x against RT x 16 of the parts * rank rows of an
-// adapter's A, over one of a.splits shares of K; its waves take 32 of K in turn.
+// adapter's A, over one of a.splits shares of K; its waves take 64 of K in turn.
 // v_mfma_f32_16x16x32_bf16 with A's rows as its rows and x's as its columns: a
 // lane ends up with four consecutive ranks of one row.
 //
 // A fragment read straight from memory is 16 bytes of each of 16 rows per
 // quarter of a wave, 16 cache lines for 256 bytes, at which the CU's cache gives
-// a quarter of its rate (8192 rows of 12800, rank 64: 94 us). Four lanes take 64
-// consecutive bytes of a row here, and a wave turns its tiles through 1 KB each
-// of LDS (the 16-byte slots of row r exchanged by r / 2, so that 8 lanes read
-// 128 bytes of different banks). DS operations of a wave execute in order, so
-// the tiles of the next 32 follow without a wait.
+// a quarter of its rate (8192 rows of 12800, rank 64: 94 us). Eight lanes take a
+// whole 128-byte line of a row here, and a wave turns its tiles through 2 KB each
+// of LDS (16-byte chunk c of row r in slot c ^ (r mod 8): 8 lanes read 128 bytes
+// of different banks). DS operations of a wave execute in order, so the tiles of
+// the next 64 follow without a wait.
 template <int RT, int XT, bool FP8>
 __global__ __launch_bounds__(kShrinkWaves * 64) __attribute__((amdgpu_waves_per_eu(RT * XT > 8 ? 2 : 4)))
 void lora_shrink_kernel(LoraArgs a) {
   constexpr int kXRows = 16 * XT;
-  constexpr int kDeep = RT + XT <= 2 ? 4 : 2;  // units in flight: 128 registers a lane
+  constexpr int kDeep = RT + XT <= 3 ? 2 : 1;  // units in flight while one is multiplied
   union Lds {
-    u32x4_t tile[kShrinkWaves][RT + XT][64];
+    u32x4_t tile[kShrinkWaves][RT + XT][128];
     f32x4_t part[kShrinkWaves][RT * XT][64];
   };
   __shared__ Lds lds;
@@ -142,13 +142,23 @@ void lora_shrink_kernel(LoraArgs a) {
   const int mine = m0 + lane < a.M && lane < kXRows ? a.adapter[m0 + lane] : -1;
   unsigned long long todo = __ballot(mine >= 0 && mine < a.adapters), done = 0ull;
   const uint8_t* xb = static_cast<const uint8_t*>(a.x);
-  const int units = a.K / 32, u_end = units * (ks + 1) / a.splits, u_first = units * ks / a.splits + wave;
-  const int lr = lane >> 2, lc = lane & 3;  // loads: row and 16-byte chunk of a tile
-  u32x4_t* const put = &lds.tile[wave][0][4 * lr + (lc ^ ((lr >> 1) & 3))];
-  const u32x4_t* const get = &lds.tile[wave][0][4 * n + (g ^ ((n >> 1) & 3))];
-  size_t xrow[XT];
+  const int units = a.K / 64, u_end = units * (ks + 1) / a.splits, u_first = units * ks / a.splits + wave;
+  const int lr = lane >> 3, lc = lane & 7;  // loads: row (and row + 8) and 16-byte chunk of a tile
+  u32x4_t* const put = &lds.tile[wave][0][8 * lr + (lc ^ lr)];
+  const u32x4_t* const get = &lds.tile[wave][0][8 * n];
+  // e4m3 rows are 64 bytes: four lanes to a row, each with two chunks of bf16.
+  const int fr = lane >> 2, fc = 2 * (lane & 3);
+  u32x4_t* const put8 = &lds.tile[wave][0][8 * fr];
+  size_t xrow[XT][FP8 ? 1 : 2];
 #pragma unroll
-  for (int j = 0; j < XT; ++j) xrow[j] = static_cast<size_t>(min(m0 + 16 * j + lr, a.M - 1)) * a.ldx + 8 * lc;
+  for (int j = 0; j < XT; ++j) {
+    if constexpr (FP8) {
+      xrow[j][0] = static_cast<size_t>(min(m0 + 16 * j + fr, a.M - 1)) * a.ldx + 16 * (lane & 3);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) xrow[j][e] = static_cast<size_t>(min(m0 + 16 * j + 8 * e + lr, a.M - 1)) * a.ldx + 8 * lc;
+    }
+  }
   for (int idx = 0; todo != 0ull; ++idx) {
     const int id = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
     const unsigned long long same = __ballot(mine == id);
@@ -161,21 +171,19 @@ void lora_shrink_kernel(LoraArgs a) {
     for (int i = 0; i < RT; ++i)
 #pragma unroll
       for (int j = 0; j < XT; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    u32x4_t xr[kDeep][XT], ar[kDeep][RT];
+    u32x4_t xr[kDeep][XT][FP8 ? 1 : 2], ar[kDeep][RT][2];
     const auto load = [&](int d, int u) {  // a unit past the end loads the last one again
-      const int k = 32 * min(u, u_end - 1);
+      const int k = 64 * min(u, u_end - 1);
 #pragma unroll
-      for (int j = 0; j < XT; ++j) {
-        if constexpr (FP8) {
-          const u32x2_t v = *reinterpret_cast<const u32x2_t*>(xb + xrow[j] + k);
-          xr[d][j] = u32x4_t{v.x, v.y, 0u, 0u};
-        } else {
-          xr[d][j] = *reinterpret_cast<const u32x4_t*>(xb + 2 * (xrow[j] + k));
-        }
-      }
+      for (int j = 0; j < XT; ++j)
+#pragma unroll
+        for (int e = 0; e < (FP8 ? 1 : 2); ++e)
+          xr[d][j][e] = *reinterpret_cast<const u32x4_t*>(xb + (FP8 ? 1 : 2) * (xrow[j][e] + k));
 #pragma unroll
       for (int i = 0; i < RT; ++i)
-        ar[d][i] = *reinterpret_cast<const u32x4_t*>(ab + static_cast<size_t>(min(r0 + 16 * i + lr, pr - 1)) * a.K + k);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          ar[d][i][e] = *reinterpret_cast<const u32x4_t*>(ab + static_cast<size_t>(min(r0 + 16 * i + 8 * e + lr, pr - 1)) * a.K + k);
     };
 #pragma unroll
     for (int d = 0; d < kDeep; ++d) load(d, u_first + d * kShrinkWaves);
@@ -186,22 +194,33 @@ void lora_shrink_kernel(LoraArgs a) {
         if (u >= u_end) break;
 #pragma unroll
         for (int j = 0; j < XT; ++j) {
-          if constexpr (FP8) put[64 * j] = fp8x8_bf16(u32x2_t{xr[d][j].x, xr[d][j].y});
-          else put[64 * j] = xr[d][j];
+          if constexpr (FP8) {
+            put8[128 * j + (fc ^ (fr & 7))] = fp8x8_bf16(u32x2_t{xr[d][j][0].x, xr[d][j][0].y});
+            put8[128 * j + ((fc + 1) ^ (fr & 7))] = fp8x8_bf16(u32x2_t{xr[d][j][0].z, xr[d][j][0].w});
+          } else {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) put[128 * j + 64 * e] = xr[d][j][e];
+          }
         }
 #pragma unroll
-        for (int i = 0; i < RT; ++i) put[64 * (XT + i)] = ar[d][i];
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) put[128 * (XT + i) + 64 * e] = ar[d][i][e];
         if (u + kDeep * kShrinkWaves < u_end) load(d, u + kDeep * kShrinkWaves);
         asm volatile("" ::: "memory");  // the reads stay behind the writes
-        bf16x8_t xf[XT];
 #pragma unroll
-        for (int j = 0; j < XT; ++j) xf[j] = __builtin_bit_cast(bf16x8_t, get[64 * j]);
+        for (int s = 0; s < 2; ++s) {
+          const int slot = (4 * s + g) ^ (n & 7);
+          bf16x8_t xf[XT];
 #pragma unroll
-        for (int i = 0; i < RT; ++i) {
-          const bf16x8_t af = __builtin_bit_cast(bf16x8_t, get[64 * (XT + i)]);
+          for (int j = 0; j < XT; ++j) xf[j] = __builtin_bit_cast(bf16x8_t, get[128 * j + slot]);
 #pragma unroll
-          for (int j = 0; j < XT; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af, xf[j], acc[i][j], 0, 0, 0);
+          for (int i = 0; i < RT; ++i) {
+            const bf16x8_t af = __builtin_bit_cast(bf16x8_t, get[128 * (XT + i) + slot]);
+#pragma unroll
+            for (int j = 0; j < XT; ++j)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af, xf[j], acc[i][j], 0, 0, 0);
+          }
         }
         asm volatile("" ::: "memory");  // and the next writes behind the reads
       }
@@ -373,7 +392,7 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraArgs a, int tiles_
 
 // How a call's shrink is cut: 16-row tiles, rank tiles of a workgroup, slots,
 // shares of K (1024 workgroups where K gives them, so that a tile with two
-// adapters is no long tail; every wave at least two units of 32).
+// adapters is no long tail; every wave at least one unit of 64).
 struct Shrink {
   int rt, xt, slots, splits;
   long long groups;  // (row tiles) x (rank groups) x slots
@@ -385,9 +404,9 @@ Shrink shrink_plan(int M, int K, int pr, int adapters) {
   // One tile's distinct adapters over workgroups of their own where rows are few.
   p.slots = M <= 64 ? std::min({16, M, adapters}) : 1;
   p.groups = static_cast<long long>((M + 16 * p.xt - 1) / (16 * p.xt)) * ((pr + 16 * p.rt - 1) / (16 * p.rt)) * p.slots;
-  const int least = M <= 64 ? 4 : 2;  // units of 32 a wave
+  const int least = M <= 64 ? 2 : 1;  // units of 64 a wave
   p.splits = static_cast<int>(std::max<long long>(
-      1, std::min<long long>({kMaxShares, 1024 / p.groups, K / (32 * kShrinkWaves * least)})));
+      1, std::min<long long>({kMaxShares, 1024 / p.groups, K / (64 * kShrinkWaves * least)})));
   return p;
 }
 // The counts' place at the start of every workspace, whatever the call: shares
