@@ -756,6 +756,9 @@ void launch_select(const SelectArgs& a, hipStream_t st) {
 
 int padded_blocks(int max_len, int block) { return ((max_len + block - 1) / block + 63) / 64 * 64; }
 
+// Whether LDS holds a row's keys and the rows fit a grid: scores then take no work.
+bool one_launch(int rows, int nbp) { return nbp <= kLdsKeys && rows <= 65535; }
+
 // Rows whose keys one launch holds: at most 64 MB of them, so that they are
 // read back from the caches.
 int slab_rows(int rows, int Hk, int nbp) {
@@ -818,6 +821,7 @@ int granite4_kv_ranges(const void* cache_k, const float* k_scale, int bits, int 
 size_t granite4_block_select_work_bytes(int rows, int Hk, int max_len, int block) {
   if (rows <= 0 || Hk <= 0 || max_len <= 0 || max_len > INT_MAX - 128 * 64 || block <= 0) return 0;
   const int nbp = padded_blocks(max_len, block);
+  if (one_launch(rows, nbp)) return 0;
   return static_cast<size_t>(slab_rows(rows, Hk, nbp)) * Hk * nbp * sizeof(uint32_t);
 }
 
@@ -829,12 +833,12 @@ int granite4_block_select(const uint16_t* q, int rows, int Hq, int Hk, int d,
   SelectArgs a{};
   a.at = RowSet{kv_base, d_pos, d_pt, row_pos, row_pt};
   const int ml = max_len > 0 ? max_len : stride;
-  if (q == nullptr || ranges == nullptr || range_scale == nullptr || work == nullptr ||
+  if (q == nullptr || ranges == nullptr || range_scale == nullptr ||
       sel == nullptr || d != kHd || Hk <= 0 || Hk > 65535 || Hq != kGq * Hk ||
       !block_ok(block, stride) || max_len < 0 || ml > stride || !row_set_ok(a.at, rows, ml) ||
       top_k < 1 || sink < 0 || recent < 1 || recent > top_k || sink > top_k - recent ||
       ml / block > 65535 * 256 - 64 || !aligned(q, 16) || !aligned(ranges, 16) ||
-      !aligned(work, 16)) {
+      !aligned(work, 16) || (work == nullptr && !one_launch(rows, padded_blocks(ml, block)))) {
     std::fprintf(stderr, "granite4: granite4_block_select: invalid arguments\n");
     return -1;
   }
@@ -854,8 +858,7 @@ int granite4_block_select(const uint16_t* q, int rows, int Hq, int Hk, int d,
   a.sel = sel;
   const hipStream_t st = stream();
   const bool one_seq = row_pos == nullptr;
-  const long long groups = one_seq && rows > 1 && a.nbp <= 4096 ? (static_cast<long long>(rows) + 3) / 4 : rows;
-  if (a.nbp <= kLdsKeys && groups <= 65535) {
+  if (one_launch(rows, a.nbp)) {
     if (one_seq && rows > 1 && a.nbp <= 1024) launch_select<8, 8, 1024>(a, st);
     else if (one_seq && rows > 1 && a.nbp <= 4096) launch_select<16, 4, 4096>(a, st);
     else if (a.nbp <= 4096) launch_select<16, 1, 4096>(a, st);

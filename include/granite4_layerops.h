@@ -606,8 +606,10 @@ int granite4_kv_ranges(const void* cache_k, const float* k_scale, int bits, int 
  * ranges (granite4_kv_ranges: off the arena, or beginning inside an arena
  * block) are never listed. sink + recent <= top_k. max_len (0: stride) bounds
  * the positions and sizes the work; positions behind it are clamped to it.
- * work: granite4_block_select_work_bytes(rows, Hk, max_len, block) bytes (at
- * most 64 MB but for contexts whose 16 rows need more), one call at a time. */
+ * work: granite4_block_select_work_bytes(rows, Hk, max_len, block) bytes, one
+ * call at a time: 0 (work may then be NULL) up to 16384 blocks and 65535 rows,
+ * where one launch keeps a row's scores on chip; else at most 64 MB but for
+ * contexts whose 16 rows need more. */
 size_t granite4_block_select_work_bytes(int rows, int Hk, int max_len, int block);
 int granite4_block_select(const uint16_t* q, int rows, int Hq, int Hk, int d,
                           const int8_t* ranges, const float* range_scale, int stride, int block,

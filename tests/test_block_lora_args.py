@@ -29,7 +29,8 @@ BAD = [
         dict(rows=-1), dict(base_pos=-1), dict(base_pos=961), dict(base_pos=2**31 - 1),
         dict(row_pos=P16), dict(row_pt=P16), dict(cache_k=P24), dict(ranges=P24)]),
     ("granite4_block_select", SELECT, [
-        dict(q=None), dict(ranges=None), dict(range_scale=None), dict(work=None), dict(sel=None),
+        dict(q=None), dict(ranges=None), dict(range_scale=None), dict(sel=None),
+        dict(work=None, stride=1 << 20, block=16), dict(work=None, rows=65536, stride=1 << 17),
         dict(d=64), dict(Hk=0, Hq=0), dict(Hq=24), dict(block=24), dict(stride=1016),
         dict(max_len=-1), dict(max_len=1025), dict(max_len=3), dict(rows=0), dict(kv_base=1021),
         dict(kv_base=-1), dict(top_k=0), dict(sink=-1), dict(recent=0), dict(sink=7),
@@ -73,8 +74,9 @@ def test_a_call_that_completes_no_block_launches_nothing():
 
 def test_workspace_sizes():
     f = L.lib.granite4_block_select_work_bytes
-    assert f(1, 8, 65536, 64) == 8 * 1024 * 4
-    assert f(4, 8, 1, 16) == 4 * 8 * 64 * 4
+    assert f(1, 8, 65536, 64) == f(65535, 8, 16384 * 16, 16) == 0  # kept on chip
+    assert f(1, 8, 16384 * 16 + 1, 16) == 8 * (16384 + 64) * 4
+    assert f(4, 8, 1 << 20, 16) == 4 * 8 * 65536 * 4
     assert f(100000, 8, 65536, 64) <= 64 << 20      # rows beyond are made in turns
     assert f(100000, 8, 65536, 64) > 60 << 20
     assert f(16, 64, 1 << 20, 16) == 16 * 64 * 65536 * 4  # but 16 rows at a time at least
