@@ -46,7 +46,7 @@ struct BlocksArgs {
   const float* ksc;    // [Hk][stride][128 / group]
   const float* vsc;
   float scale2;        // scale * log2(e)
-  int Hk, stride, rows;
+  int Hk, stride, first, rows;  // this launch's rows: first .. rows - 1
   RowSet at;
   const int32_t* sel;  // [rows][Hk][top_k]
   int top_k, log_block, splits;
@@ -129,7 +129,7 @@ void attn_blocks_kernel(BlocksArgs a) {
   auto vsc_at = [&](int key, int gi) -> float& { return vlf[key * (kVPitch / 2) + kHd / 2 + 4 + gi]; };
   const int g = lane >> 4, n = lane & 15;
   const int h = blockIdx.x, split = blockIdx.z;
-  const int row = blockIdx.y;
+  const int row = a.first + blockIdx.y;
   const bool live = n < kGq;
   const long long pos = row_position(a.at, row);
   const int* pt = row_table(a.at, row);
@@ -440,17 +440,18 @@ int granite4_attn_blocks(const uint16_t* q, int rows, int Hq, int Hk, int d, flo
   a.log_block = block == 16 ? 4 : block == 32 ? 5 : block == 64 ? 6 : 7;
   a.splits = blocks_splits(rows, Hk, top_k, block);  // 1 from 64 rows of 8 KV heads on
   const hipStream_t st = stream();
-  for (int r0 = 0; r0 < rows; r0 += kSlab) {
-    a.rows = std::min(kSlab, rows - r0);
-    a.q = q + static_cast<size_t>(r0) * Hq * kHd;
-    a.sel = sel + static_cast<size_t>(r0) * Hk * top_k;
-    a.out = out + static_cast<size_t>(r0) * Hq * kHd;
-    if (a.splits > 1) {  // one slab
-      a.arrived = static_cast<unsigned*>(scratch);
-      a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(scratch) + kArrivedBytes);
-      a.part_o = reinterpret_cast<float*>(a.part_ml + static_cast<size_t>(a.rows) * Hq * a.splits);
-    }
-    const dim3 grid(Hk, a.rows, a.splits);
+  a.q = q;
+  a.sel = sel;
+  a.out = out;
+  if (a.splits > 1) {  // below 512 (row, KV head) pairs: one launch
+    a.arrived = static_cast<unsigned*>(scratch);
+    a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(scratch) + kArrivedBytes);
+    a.part_o = reinterpret_cast<float*>(a.part_ml + static_cast<size_t>(rows) * Hq * a.splits);
+  }
+  for (int r0 = 0; r0 < rows; r0 += std::min(kSlab, rows - r0)) {
+    a.first = r0;
+    a.rows = r0 + std::min(kSlab, rows - r0);
+    const dim3 grid(Hk, a.rows - r0, a.splits);
     switch (bits) {
       case 16: launch_blocks<16>(a, group, grid, st); break;
       case 8: launch_blocks<8>(a, group, grid, st); break;

@@ -359,6 +359,19 @@ def test_attend_not_finite(bits, group):
         assert bad[:, 4:, 5].all() and bad[1, 3].all() and bad.sum() == D + 8
 
 
+@pytest.mark.parametrize("bits", [16, 4])
+def test_attend_rows_of_two_launches(bits):
+    """More rows than one launch has: each at its own position still."""
+    rows, base, group = 65537 + 70, 40, 128
+    P = Pool(bits, group, 1, 65536 + 256, 64, 80 + bits)
+    pos = base + np.arange(rows)
+    sel = np.stack([pos // 64, pos // 128 - 1], -1).astype(np.int32)[:, None]
+    q = queries(P.rng, rows, 1)
+    got = P.attend(q, sel, 0.125, base)
+    at = np.array([0, 1, 100, 65534, 65535, 65536, 65537, rows - 2, rows - 1])
+    P.check(got[at], q[at], sel[at], pos[at], [np.arange(P.stride)] * len(at), 0.125)
+
+
 def test_attend_large_logits():
     """Logits in the hundreds, of either sign: the running maximum holds."""
     P = Pool(16, 128, 2, 1024, 64, 71)
