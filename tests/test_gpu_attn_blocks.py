@@ -372,6 +372,62 @@ def test_attend_rows_of_two_launches(bits):
     P.check(got[at], q[at], sel[at], pos[at], [np.arange(P.stride)] * len(at), 0.125)
 
 
+@pytest.mark.parametrize("rows,Hk,block,top_k", [(512, 2, 64, 5), (300, 8, 64, 9), (601, 8, 128, 3), (790, 8, 64, 70)])
+@pytest.mark.parametrize("side", ["together", "apart"])
+def test_attend_rows_together(rows, Hk, block, top_k, side):
+    """bf16 rows of one sequence that share a wave (one to four of them): lists in any
+    order, with entries behind the row, negative, repeated and shared with the next
+    row; arena rows side by side or apart, some keys without one; the position on the
+    device."""
+    P = Pool(16, 128, Hk, 8192, block, rows + top_k)
+    pt = ref.table(P.rng, 8192 // block, block) if side == "together" else P.rng.permutation(8192).astype(np.int32)
+    pt[5 * block + 3] = -1
+    pt[7 * block:8 * block] = 8192
+    start = 4000
+    pos = start + np.arange(rows)
+    q = queries(P.rng, rows, Hk)
+    sel = random_lists(P.rng, pos, Hk, top_k, block)
+    at = np.r_[0:8, 130:142, rows - 9:rows]
+    sel[at[0]] = -1
+    sel[at[1], 0] = 8192 // block - 1             # behind the row, every entry
+    sel[at[2]] = sel[at[2]][:, ::-1]              # descending, the -1 first
+    sel[at[3], 1, 1:3] = sel[at[3], 1, 0]         # counted three times
+    sel[at[4]:at[6], 0] = sel[at[4], 0]           # two rows alike
+    sel[at[6], 0, :2] = [2**31 - 1, -2**31]
+    sel[at[9]:at[9] + 4] = sel[at[9]]             # four rows alike
+    sel[at[15], 0, 0] = 7                         # no key with a row
+    sel[at[-1], 0] = np.where(np.arange(top_k) == top_k - 1, 5, -1)
+    d_pos = dev(np.array([start], np.int32)) if side == "apart" else None
+    got = P.attend(q, sel, 1 / 16, 0 if side == "apart" else start, dev(pt), d_pos)
+    P.check(got[at], q[at], sel[at], pos[at], [pt] * len(at), 1 / 16)
+    assert (got[at[0]] == 0).all() and (got[at[1], :4] == 0).all()
+
+
+def test_attend_rows_together_garbage():
+    """What a row does not list or see does not reach it from the rows beside it."""
+    P = Pool(16, 128, 8, 2048, 64, 83)
+    rows, start = 520, 1000
+    pos = start + np.arange(rows)
+    q = queries(P.rng, rows, 8)
+    sel = random_lists(P.rng, pos, 8, 6, 64)
+    want = P.attend(q, sel, 0.25, start)
+    at = np.r_[0:6, 400:406, 514:520]
+    P.check(want[at], q[at], sel[at], pos[at], [np.arange(2048)] * len(at), 0.25)
+    for t in (P.k, P.v):  # NaN in block 3, infinity behind the last row
+        x = t.view(torch.int16).view(8, 2048, D)
+        x[:, 192:256] = 0x7FC0
+        x[:, start + rows:] = 0x7F80
+    listed = np.repeat((sel == 3).any(-1), 4, 1)
+    assert listed.any() and not listed.all()
+    got = P.attend(q, sel, 0.25, start)
+    np.testing.assert_array_equal(got[~listed], want[~listed])
+    # the last row sees its own key last
+    q[9, 2 * D + 1] = 0x7FC0
+    bad = np.isnan(ref.f32(P.attend(q, sel, 0.25, start)))
+    clean = ~listed
+    assert bad[9, 2].all() and bad[clean].sum() == (D if clean[9, 2] else 0)
+
+
 def test_attend_large_logits():
     """Logits in the hundreds, of either sign: the running maximum holds."""
     P = Pool(16, 128, 2, 1024, 64, 71)
