@@ -672,7 +672,7 @@ void attn_blocks_merged_kernel(BlocksArgs a, int per_wave) {
     const float alpha = exp2_hw(m - base);
     m = mx;
     l *= alpha;
-    if (__any(alpha != 1.0f)) {
+    if (__any(takes && alpha != 1.0f)) {  // the others' is 1, or 0 with sums of 0
 #pragma unroll
       for (int nb = 0; nb < 8; ++nb) o[nb] *= alpha;
     }

@@ -403,6 +403,28 @@ def test_attend_rows_together(rows, Hk, block, top_k, side):
     assert (got[at[0]] == 0).all() and (got[at[1], :4] == 0).all()
 
 
+@pytest.mark.parametrize("bits,group", [(16, 128), (8, 128), (4, 32), (5, 64)])
+@pytest.mark.parametrize("rows,block", [(254, 32), (511, 16)])
+def test_attend_many_sequences(bits, group, rows, block):
+    """A wave for each row: rows of sequences with tables of their own, their lists
+    in any order."""
+    P = Pool(bits, group, 8, 4096, block, rows + bits)
+    pts = [ref.table(P.rng, 4096 // block, block) for _ in range(3)] + [np.arange(4096, dtype=np.int32)]
+    pts[1][2 * block + 1] = -1
+    pos = P.rng.integers(0, 4096, rows).astype(np.int32)
+    pos[:4] = -1, 0, 4095, 5
+    q = queries(P.rng, rows, 8)
+    sel = random_lists(P.rng, np.maximum(pos, 0), 8, 7, block)
+    sel[4] = sel[4][:, ::-1]
+    sel[5, 2] = -1
+    sel[6, 1, 3] = 4096 // block - 1
+    d = [dev(t) for t in pts[:3]] + [None]
+    got = P.attend(q, sel, 1 / 16, row_pos=dev(pos), row_pt=ptrs([d[r % 4] for r in range(rows)]))
+    at = np.r_[0:12, rows - 6:rows]
+    P.check(got[at], q[at], sel[at], pos[at], [pts[r % 4] for r in at], 1 / 16)
+    assert (got[0] == 0).all() and (got[5, 8:12] == 0).all()
+
+
 def test_attend_rows_together_garbage():
     """What a row does not list or see does not reach it from the rows beside it."""
     P = Pool(16, 128, 8, 2048, 64, 83)
