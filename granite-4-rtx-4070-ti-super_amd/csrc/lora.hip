@@ -36,7 +36,7 @@ typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
 
 constexpr int kMaxRank = 128;
 constexpr int kShrinkWaves = 8;
-constexpr int kMaxShares = 8;  // of K
+constexpr int kMaxShares = 8;  // of K: the shrink's join has that many loads
 
 struct LoraArgs {
   const void* x;          // [M][ldx] bf16, or e4m3 codes under *xs
@@ -165,6 +165,12 @@ void lora_shrink_kernel(LoraArgs a) {
     todo &= ~same;
     if (idx % static_cast<int>(gridDim.z) != static_cast<int>(blockIdx.z)) continue;
     done |= same;
+    // 16-row tiles of x that have a row of this adapter: a tile on the border of two
+    // sessions multiplies each part with its own adapter's A only.
+    unsigned need = 0u;
+#pragma unroll
+    for (int j = 0; j < XT; ++j) need |= static_cast<unsigned>(((same >> (16 * j)) & 0xffffull) != 0ull) << j;
+    const auto needs = [&](int j) { return XT == 1 || ((need >> j) & 1u) != 0u; };
     const uint16_t* ab = a.A + static_cast<size_t>(id) * pr * a.K + 8 * lc;
     f32x4_t acc[RT][XT];
 #pragma unroll
@@ -175,10 +181,12 @@ void lora_shrink_kernel(LoraArgs a) {
     const auto load = [&](int d, int u) {  // a unit past the end loads the last one again
       const int k = 64 * min(u, u_end - 1);
 #pragma unroll
-      for (int j = 0; j < XT; ++j)
+      for (int j = 0; j < XT; ++j) {
+        if (!needs(j)) continue;
 #pragma unroll
         for (int e = 0; e < (FP8 ? 1 : 2); ++e)
           xr[d][j][e] = *reinterpret_cast<const u32x4_t*>(xb + (FP8 ? 1 : 2) * (xrow[j][e] + k));
+      }
 #pragma unroll
       for (int i = 0; i < RT; ++i)
 #pragma unroll
@@ -194,6 +202,7 @@ void lora_shrink_kernel(LoraArgs a) {
         if (u >= u_end) break;
 #pragma unroll
         for (int j = 0; j < XT; ++j) {
+          if (!needs(j)) continue;
           if constexpr (FP8) {
             put8[128 * j + (fc ^ (fr & 7))] = fp8x8_bf16(u32x2_t{xr[d][j][0].x, xr[d][j][0].y});
             put8[128 * j + ((fc + 1) ^ (fr & 7))] = fp8x8_bf16(u32x2_t{xr[d][j][0].z, xr[d][j][0].w});
@@ -213,13 +222,14 @@ void lora_shrink_kernel(LoraArgs a) {
           const int slot = (4 * s + g) ^ (n & 7);
           bf16x8_t xf[XT];
 #pragma unroll
-          for (int j = 0; j < XT; ++j) xf[j] = __builtin_bit_cast(bf16x8_t, get[128 * j + slot]);
+          for (int j = 0; j < XT; ++j)
+            if (needs(j)) xf[j] = __builtin_bit_cast(bf16x8_t, get[128 * j + slot]);
 #pragma unroll
           for (int i = 0; i < RT; ++i) {
             const bf16x8_t af = __builtin_bit_cast(bf16x8_t, get[128 * (XT + i) + slot]);
 #pragma unroll
             for (int j = 0; j < XT; ++j)
-              acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af, xf[j], acc[i][j], 0, 0, 0);
+              if (needs(j)) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af, xf[j], acc[i][j], 0, 0, 0);
           }
         }
         asm volatile("" ::: "memory");  // and the next writes behind the reads
@@ -257,9 +267,11 @@ void lora_shrink_kernel(LoraArgs a) {
     const int at = e & (kXRows - 1), r = r0 + 4 * (e / kXRows);
     if (((done >> at) & 1ull) == 0ull || r >= pr) continue;
     const float* src = a.part + static_cast<size_t>(m0 + at) * pr + r;
-    f32x4_t p[kMaxShares];
-#pragma unroll
-    for (int k = 0; k < kMaxShares; ++k) p[k] = ld_dev(src + static_cast<size_t>(min(k, a.splits - 1)) * a.M * pr);
+    f32x4_t p[kMaxShares];  // two, four or all eight loads under way at once
+    const auto load = [&](int k) { p[k] = ld_dev(src + static_cast<size_t>(min(k, a.splits - 1)) * a.M * pr); };
+    load(0), load(1);
+    if (XT == 1 || a.splits > 2) load(2), load(3);
+    if (XT == 1 || a.splits > 4) load(4), load(5), load(6), load(7);
     f32x4_t v = p[0];
 #pragma unroll
     for (int k = 1; k < kMaxShares; ++k)
@@ -390,9 +402,7 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraArgs a, int tiles_
   }
 }
 
-// How a call's shrink is cut: 16-row tiles, rank tiles of a workgroup, slots,
-// shares of K (1024 workgroups where K gives them, so that a tile with two
-// adapters is no long tail; every wave at least one unit of 64).
+// How a call's shrink is cut: 16-row tiles, rank tiles of a workgroup, slots, shares of K.
 struct Shrink {
   int rt, xt, slots, splits;
   long long groups;  // (row tiles) x (rank groups) x slots
@@ -404,9 +414,24 @@ Shrink shrink_plan(int M, int K, int pr, int adapters) {
   // One tile's distinct adapters over workgroups of their own where rows are few.
   p.slots = M <= 64 ? std::min({16, M, adapters}) : 1;
   p.groups = static_cast<long long>((M + 16 * p.xt - 1) / (16 * p.xt)) * ((pr + 16 * p.rt - 1) / (16 * p.rt)) * p.slots;
-  const int least = M <= 64 ? 2 : 1;  // units of 64 a wave
-  p.splits = static_cast<int>(std::max<long long>(
-      1, std::min<long long>({kMaxShares, 1024 / p.groups, K / (64 * kShrinkWaves * least)})));
+  const int units = K / (64 * kShrinkWaves);  // of 64, a wave's, in one share
+  if (M <= 64) {  // 1024 workgroups where K gives them, every wave two units
+    p.splits = static_cast<int>(std::max<long long>(1, std::min<long long>({kMaxShares, 1024 / p.groups, units / 2})));
+    return p;
+  }
+  // Workgroups run in rounds of what the CUs hold, one each of the forms with four
+  // rank tiles (registers) and two of the others. A workgroup's time is its share's
+  // units and, about three units of each wave, its start, joins in LDS and sums to
+  // memory: the number of shares that makes the least of rounds times that. us a call
+  // with 1024 workgroups wherever K gives them and with the rule: 8192 x 12800 rank 64, 128 groups, 8 and 2 shares 124 and 105; 4096 rows
+  // 78 and 66 (8, 4); 8192 x 4096, ranks 3 x 16, 89 and 68 (8, 2); 2048 rows, 3 x 32, 44 and 31.
+  p.splits = 1;
+  const long long held = p.rt == 4 ? kCUs : 2 * kCUs;
+  long long least = LLONG_MAX;
+  for (int s = 1; s <= std::min(kMaxShares, units) && (s == 1 || s * p.groups <= 1024); ++s) {
+    const long long time = (s * p.groups + held - 1) / held * (K / 64 / s + 3 * kShrinkWaves);
+    if (time < least) least = time, p.splits = s;
+  }
   return p;
 }
 // The counts' place at the start of every workspace, whatever the call: shares
@@ -508,9 +533,9 @@ int granite4_lora_add(int out, const void* X, int x_bits, int ldx, const float* 
   else if (plan.xt == 2) launch_shrink<4, 2>(a, fp8, 1, st);
   else launch_shrink<4, 4>(a, fp8, 1, st);
   // Row tiles of a wave: one where its columns of B are small beside the tile (rank
-  // 16: 1001 x 25600 f32 49.6 us against 53.7 with four), else as many, up to
-  // eight, as leave every CU four workgroups (rank 64, 8192 x 4096: 123 us the call
-  // with eight, 130 with four, 139 with one).
+  // 16: 1001 x 25600 f32 50 us against 55 with six), else as many, up to eight, as
+  // leave every CU four workgroups (rank 64, 8192 x 4096: 105 us the call with
+  // eight, 112 with four, 121 with one).
   const long long wgs = static_cast<long long>((M + 15) / 16) * ((N + 255) / 256);
   const int per = rank <= 32 ? 1 : static_cast<int>(std::clamp<long long>(wgs / (4 * kCUs), 1, 8));
   const bool f32 = out == GRANITE4_GEMM_F32;

@@ -117,6 +117,19 @@ def test_lora(M, N, K, rank, count, segs, fp8, f32):
     c.check(c.run(0.22), 0.22)
 
 
+@pytest.mark.parametrize("M,K,rank", [(4113, 1600, 40), (4100, 64, 64), (4230, 320, 16), (300, 1088, 72), (150, 640, 24)])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_lora_of_sessions_in_runs(M, K, rank, fp8):
+    """Rows of a few sessions one after another, as a chunk has them: borders inside
+    and at the ends of 16- and 64-row tiles, runs of one row, rows without an adapter."""
+    c = Case(M, 72, K, rank, 5, fp8=fp8)
+    c.adapter[:] = -1
+    at = [0, 16, 33, 34, 80, 128, 135, 144, M - 70, M - 64, M - 17, M - 1, M]
+    for i, (lo, hi) in enumerate(zip(at, at[1:])):
+        c.adapter[lo:hi] = (3 * i) % 7 - 1  # -1 .. 5: none, 0 .. 4, out of range
+    c.check(c.run(0.5), 0.5)
+
+
 @pytest.mark.parametrize("M", [3, 40, 270])
 @pytest.mark.parametrize("f32", [False, True])
 def test_lora_without_base_and_in_place(M, f32):
