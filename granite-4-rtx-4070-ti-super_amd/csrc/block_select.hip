@@ -48,7 +48,9 @@ __device__ __forceinline__ float col_min4(float x) { return -col_max4(-x); }
 // One wave per (unit, KV head): 16 lanes cover a key's 128 channels (8 each),
 // four keys at a time, every load of the block in flight before the first use.
 // A unit is a block of the call's positions, or (row_pos) a row, whose block
-// counts where the row's position is its last.
+// counts where the row's position is its last. The table, the keys and the reduction
+// wait for one another, and that is its time: 500 rows of bf16 in blocks of 32 with 8
+// KV heads 4.6 us, 8192 rows of K5 in groups of 32 in blocks of 64 7.8 (unpacking).
 template <int BITS, int GROUP, int BLOCK>
 __global__ __launch_bounds__(256) void kv_ranges_kernel(RangeArgs a) {
   constexpr int kKb = k_row_bytes(BITS);
@@ -604,6 +606,10 @@ struct WidePick {
 
 // One workgroup per (ROWS rows, KV head): scores into LDS, then one wave per
 // row (all waves for one row) lists its blocks. KEYS: keys of a row that fit.
+// 8 KV heads, blocks of 64, 32 listed: one row among 470 blocks 8.1 us a call (table,
+// ranges, scores, limit and list in turn), 1000 rows among 900 31.7 (8000 limits and
+// lists by one wave each, and the scores' f32 steps); 16 sessions, blocks of 32, 64 of
+// up to 2031 listed, 13 to 15 (the longest session's blocks by one CU per KV head).
 template <int W, int ROWS, int KEYS>
 __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(4))) void block_select_kernel(SelectArgs a) {
   using S = Scorer<W, ROWS>;
